@@ -23,7 +23,8 @@
  * as the driver's are; there is no global state beyond the context, with one
  * exception: emb_array_sum_f32_static keeps a device array per GPU and a
  * process-wide table of its addresses, and, being written against the CUDA
- * runtime, returns cudaError_t values (> 0) where the others return CUresult.
+ * runtime, returns cudaError_t values (> 0) where the others return CUresult
+ * (so do the emb_paged_* operators).
  */
 #ifndef EMMY_B200_H
 #define EMMY_B200_H
@@ -176,6 +177,143 @@ typedef struct {
     uint32_t wait_limit_us;       /* e.g. 2000000 */
     uint32_t reserved;            /* 0 */
 } emb_peer_exchange_t;
+
+/* ---- the serving step over a paged key-value cache -----------------------------
+ * Library operators, like emb_array_sum_f32_static: run-time sizes, no IR behind
+ * them, no counterpart in the reference (its attention is over whole prompts of
+ * compile-time length). A step of a server calls them in this order:
+ * emb_paged_assign gives the step's new tokens their places in the cache,
+ * emb_paged_store normalises and rotates the new queries and keys and stores keys
+ * and values there, emb_paged_attend attends one new token of each request over
+ * its pages (a prompt's own rows go through the attention family).
+ *
+ * Every pointer is a device address on the current device; the caller owns all of
+ * them. Strides are in elements. Calls are asynchronous on `stream`, allocate
+ * nothing, read nothing back and may be captured into a CUDA graph. Arguments that
+ * the host can judge are refused with EMB_E_ARGUMENT and a text before anything is
+ * launched; what only the device can see is stated at each call. Like
+ * emb_array_sum_f32_static they return cudaError_t values (> 0) when a launch is
+ * refused. */
+
+/* The pages of a cache: element (page, token, head, d) of the keys is
+ * k[page * k_stride[0] + token * k_stride[1] + head * k_stride[2] + d], of the
+ * values likewise; so pages may be token-major or head-major, and keys and values
+ * parts of one buffer. A SLOT is page * page_size + token. */
+typedef struct {
+    void* k;
+    void* v;
+    int64_t k_stride[3]; /* page, token, head: multiples of 16 bytes */
+    int64_t v_stride[3];
+    int32_t pages;     /* >= 1; pages * page_size < 2^31 */
+    int32_t page_size; /* tokens in a page, >= 1, any number */
+    int32_t kv_heads;
+    int32_t dim;     /* 64, 128 or 256 */
+    int32_t dtype;   /* EMB_F16, EMB_BF16, or EMB_U8: e4m3 codes */
+    float k_scale;   /* of e4m3 codes: value = code * scale; else 1 */
+    float v_scale;
+    int32_t reserved; /* 0 */
+} emb_paged_cache_t;
+
+/* Page tables and slot maps of one step. Request b has cached[b] tokens in the
+ * cache and brings fresh[b] new ones (negative counts as 0); its new tokens are
+ * the step's rows starts[b] .. starts[b+1]-1. The pages they need beyond those
+ * that hold cached[b] tokens come from free_pages[*free_head ..] in the order of
+ * the requests and are entered into the request's row of `table`, whose other
+ * entries are left as they are.
+ *   slots[i], positions[i]   row i's slot and position in its request; -1 and 0 in
+ *                            the rows behind the last request
+ *   starts[requests + 1]     prefix sums of fresh
+ *   lengths[b]               cached[b] + fresh[b]
+ *   free_head_out            *free_head + pages taken
+ *   report[4]                pages taken, requests refused, rows wanted beyond
+ *                            `tokens`, rows wanted
+ * A request is refused whole when its tokens do not fit its table row or the
+ * step's `tokens` rows, or when the free pages end before its need and the need of
+ * the requests before it: its slots are -1, its length stays cached[b], its table
+ * row stays as it is. An entry of the table that is negative gives slot -1.
+ * Outputs may not share memory with inputs (but for `table`). */
+typedef struct {
+    const int32_t* cached;
+    const int32_t* fresh;
+    int32_t* table;
+    const int32_t* free_pages;
+    const int32_t* free_head;
+    int32_t* slots;
+    int32_t* positions;
+    int32_t* starts;
+    int32_t* lengths;
+    int32_t* free_head_out;
+    int32_t* report;
+    int64_t table_stride; /* of a request's row */
+    int32_t requests;
+    int32_t table_width;
+    int32_t free_count; /* entries of free_pages */
+    int32_t page_size;
+    int32_t tokens; /* rows of slots and positions */
+    int32_t reserved; /* 0 */
+} emb_paged_assign_t;
+int emb_paged_assign(const emb_paged_assign_t* args, void* stream);
+
+/* Norm, rotation and store of a step's rows, in one pass:
+ *   x  = q[i, h] or k[i, h];  y = x / sqrt(mean(x^2) + eps) * weight   (weight NULL: y = x)
+ *   rotation of the first `rot` dims by the angles of positions[i]: rope holds, for
+ *   each position, rot/2 cosines and then rot/2 sines; pair j is (y[j], y[j+rot/2]),
+ *   or (y[2j], y[2j+1]) where `interleaved`:  (a c - b s, b c + a s)
+ * all in f32, rounded once: q_out[i, h] in q's type, keys and values (the values as
+ * they are) into slot slots[i] of the cache in the cache's type (e4m3: divided by
+ * the scale, nearest even, saturating). A slot outside the cache (negative among
+ * them) stores nothing; its q_out is written. A position outside the table gives
+ * NaN in the rotated dims. Two rows with the same slot: either's values. q_out may
+ * be q. A cache of 16-bit type has q's type. */
+typedef struct {
+    const void* q; /* [tokens, heads, dim], q_stride = row, head */
+    const void* k; /* [tokens, kv_heads, dim] */
+    const void* v;
+    void* q_out;
+    const int32_t* slots;
+    const int32_t* positions; /* may be NULL where rot is 0 */
+    const float* rope;        /* [rope_rows, rot] contiguous, 16-byte aligned; NULL where rot is 0 */
+    const void* q_weight;     /* [dim] of q's type, or NULL */
+    const void* k_weight;
+    emb_paged_cache_t cache;
+    int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2];
+    int32_t tokens, heads;
+    int32_t dtype; /* EMB_F16 or EMB_BF16 */
+    int32_t rot;   /* 0, or a multiple of 16 up to dim */
+    int32_t rope_rows;
+    int32_t interleaved;
+    float eps;
+    int32_t reserved; /* 0 */
+} emb_paged_store_t;
+int emb_paged_store(const emb_paged_store_t* args, void* stream);
+
+/* Attention of one token of each request over its pages:
+ *   out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j,  j in [max(0, L - window), L),
+ *   L = lengths[b] (negative counts as 0; window 0: all), key head h / (heads / kv_heads)
+ * Key j is token j % page_size of page table[b, j / page_size]. A row without keys
+ * gives 0 (lse: -inf). What pages hold behind a request's length is not looked at
+ * (NaN there does no harm). A table entry outside the cache, and a length beyond
+ * the table row, give NaN in the request's outputs. Scores, their maximum and sum
+ * and the output are held in f32; the weights are rounded to 16 bits (q's type;
+ * f16 over an e4m3 cache) for the product with the values.
+ *   lse[b, h]  natural logarithm of the sum of exponentials, f32, contiguous; or NULL
+ * A cache of 16-bit type has q's type. */
+typedef struct {
+    const void* q; /* [requests, heads, dim], q_stride = request, head */
+    void* out;
+    float* lse;
+    const int32_t* table;
+    const int32_t* lengths;
+    emb_paged_cache_t cache;
+    int64_t q_stride[2], out_stride[2];
+    int64_t table_stride;
+    int32_t requests, heads;
+    int32_t table_width;
+    int32_t dtype; /* EMB_F16 or EMB_BF16 */
+    int32_t window;
+    float scale;
+} emb_paged_attend_t;
+int emb_paged_attend(const emb_paged_attend_t* args, void* stream);
 
 /* Text of the last error on the calling thread ("" if none). */
 const char* emb_last_error(void);
