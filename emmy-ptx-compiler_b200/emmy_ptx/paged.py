@@ -23,7 +23,7 @@ from . import driver
 _CACHE = "QQ 3q 3q iiii i ff i"
 _ASSIGN = struct.Struct("@ QQQQQQQQQQQ q iiii i i".replace(" ", ""))
 _STORE = struct.Struct(("@ QQQQQQQQQ" + _CACHE + "2q 2q 2q 2q ii i i i i f i").replace(" ", ""))
-_ATTEND = struct.Struct(("@ QQQQQ" + _CACHE + "2q 2q q ii i i i f").replace(" ", ""))
+_ATTEND = struct.Struct(("@ QQQQQQ" + _CACHE + "2q 2q q q ii i i i f").replace(" ", ""))
 
 _CODE = {torch.float8_e4m3fn: 0, torch.float16: 1, torch.bfloat16: 2}
 _BYTES = {0: 1, 1: 2, 2: 2}
@@ -213,7 +213,15 @@ def attend(q, k_pages, v_pages, table, lengths, scale: float | None = None, wind
         lse_at = lse.data_ptr()
     device = q.get_device()
     _same_device("attend", device, k_pages, v_pages, table, lengths, out, lse)
-    _call(driver.library().emb_paged_attend, device, _ATTEND.pack(
-        q.data_ptr(), out.data_ptr(), lse_at, table.data_ptr(), lengths.data_ptr(), *cache, *q_stride, *out_stride,
-        table.stride(0), requests, heads, table.shape[1], _CODE[dtype], window, dim ** -0.5 if scale is None else scale))
+    lib = driver.library()
+    fields = [q.data_ptr(), out.data_ptr(), lse_at, table.data_ptr(), lengths.data_ptr(), 0, *cache, *q_stride, *out_stride,
+              table.stride(0), 0, requests, heads, table.shape[1], _CODE[dtype], window, dim ** -0.5 if scale is None else scale]
+    if device >= 0:
+        with torch.cuda.device(device):
+            need = lib.emb_paged_attend_workspace(_ATTEND.pack(*fields))
+        if need < 0:
+            driver.check(need)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        fields[5], fields[-7] = workspace.data_ptr(), need
+    _call(lib.emb_paged_attend, device, _ATTEND.pack(*fields))
     return out

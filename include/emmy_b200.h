@@ -304,9 +304,11 @@ typedef struct {
     float* lse;
     const int32_t* table;
     const int32_t* lengths;
+    void* workspace; /* at least emb_paged_attend_workspace bytes, 16-byte aligned, of any content; one call at a time */
     emb_paged_cache_t cache;
     int64_t q_stride[2], out_stride[2];
     int64_t table_stride;
+    int64_t workspace_bytes;
     int32_t requests, heads;
     int32_t table_width;
     int32_t dtype; /* EMB_F16 or EMB_BF16 */
@@ -314,6 +316,10 @@ typedef struct {
     float scale;
 } emb_paged_attend_t;
 int emb_paged_attend(const emb_paged_attend_t* args, void* stream);
+/* The bytes of workspace that a call with these sizes and types needs on the current
+ * device (pointers and strides of q, out, table and the workspace are not looked
+ * at); negative: an error. It does not depend on what the lengths hold. */
+int64_t emb_paged_attend_workspace(const emb_paged_attend_t* args);
 
 /* Text of the last error on the calling thread ("" if none). */
 const char* emb_last_error(void);

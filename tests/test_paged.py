@@ -39,7 +39,7 @@ int main() {
     cache = (5, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1.0, 1.0, 0)
     pack = paged._STORE.pack(*[0] * 9, *cache, *[0] * 8, 0, 0, 0, 0, 0, 0, 0.5, 0)
     assert pack[out[4]] == 5 and pack[out[5]:out[5] + 4] == b"\x00\x00\x00\x3f"
-    pack = paged._ATTEND.pack(*[0] * 5, *cache, *[0] * 4, 9, 0, 0, 0, 0, 0, 0.5)
+    pack = paged._ATTEND.pack(*[0] * 6, *cache, *[0] * 4, 9, 0, 0, 0, 0, 0, 0, 0.5)
     assert pack[out[6]] == 5 and pack[out[7]] == 9 and pack[out[8]:out[8] + 4] == b"\x00\x00\x00\x3f"
 
 
@@ -130,7 +130,7 @@ def cache_fields(**kw):
 
 
 def attend_fields(cache=(), **kw):
-    f = dict(q=A, out=A, lse=0, table=A, lengths=A, cache=cache_fields(**dict(cache)), q0=256, q1=64, o0=256, o1=64, ts=2, requests=3, heads=4,
+    f = dict(q=A, out=A, lse=0, table=A, lengths=A, ws=A, cache=cache_fields(**dict(cache)), q0=256, q1=64, o0=256, o1=64, ts=2, wb=1 << 30, requests=3, heads=4,
              width=2, dtype=1, window=0, scale=0.125)
     f.update(kw)
     return [x for v in f.values() for x in (v if isinstance(v, list) else [v])]
