@@ -56,8 +56,6 @@ def library() -> ctypes.CDLL:
         lib.emb_tensor_map.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
                                        ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64),
                                        ctypes.POINTER(ctypes.c_uint32), ctypes.c_int]
-        lib.emb_paged_attend_workspace.argtypes = [ctypes.c_char_p]
-        lib.emb_paged_attend_workspace.restype = ctypes.c_int64
         _lib = lib
     return _lib
 

@@ -1,6 +1,7 @@
 """The paged-cache operators on a machine without a GPU: what they refuse, and the layout of their argument structures."""
 
 import ctypes
+import struct
 import subprocess
 from pathlib import Path
 
@@ -9,11 +10,17 @@ import torch
 
 ROOT = Path(__file__).resolve().parents[1]
 
+# the structures of include/emmy_b200.h, field by field
+CACHE = "QQ 3q 3q iiii i ff i"
+ASSIGN = struct.Struct("@QQQQQQQQQQQ q iiii i i".replace(" ", ""))
+STORE = struct.Struct(("@QQQQQQQQQ" + CACHE + "2q 2q 2q 2q ii i i i i f i").replace(" ", ""))
+ATTEND = struct.Struct(("@QQQQQQ" + CACHE + "2q 2q q q ii i i i f").replace(" ", ""))
+
 
 @pytest.fixture(scope="module")
 def paged():
     import __graft_entry__ as g
-    g.build_library()
+    g.build_binding()
     from emmy_ptx import paged
     return paged
 
@@ -32,14 +39,14 @@ int main() {
 ''')
     subprocess.run(["g++", "-I", str(ROOT / "include"), "-o", str(tmp_path / "layout"), str(src)], check=True)
     out = [int(v) for v in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()]
-    assert out[:3] == [paged._ASSIGN.size, paged._STORE.size, paged._ATTEND.size]
+    assert out[:3] == [ASSIGN.size, STORE.size, ATTEND.size]
     # a value put into each field of interest is found at the field's offset
-    pack = paged._ASSIGN.pack(*range(11), 0, 0, 0, 0, 0, 77, 0)
+    pack = ASSIGN.pack(*range(11), 0, 0, 0, 0, 0, 77, 0)
     assert int.from_bytes(pack[out[3]:out[3] + 4], "little") == 77
     cache = (5, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1.0, 1.0, 0)
-    pack = paged._STORE.pack(*[0] * 9, *cache, *[0] * 8, 0, 0, 0, 0, 0, 0, 0.5, 0)
+    pack = STORE.pack(*[0] * 9, *cache, *[0] * 8, 0, 0, 0, 0, 0, 0, 0.5, 0)
     assert pack[out[4]] == 5 and pack[out[5]:out[5] + 4] == b"\x00\x00\x00\x3f"
-    pack = paged._ATTEND.pack(*[0] * 6, *cache, *[0] * 4, 9, 0, 0, 0, 0, 0, 0, 0.5)
+    pack = ATTEND.pack(*[0] * 6, *cache, *[0] * 4, 9, 0, 0, 0, 0, 0, 0, 0.5)
     assert pack[out[6]] == 5 and pack[out[7]] == 9 and pack[out[8]:out[8] + 4] == b"\x00\x00\x00\x3f"
 
 
@@ -65,12 +72,15 @@ def refused(call, match):
 def test_attend_refuses(paged):
     k, v = pages()
     q, table, lengths = rows(), i32(3, 2), i32(3)
-    refused(lambda: paged.attend(q[0], k, v, table, lengths), r"\[requests, heads, dim\]")
-    refused(lambda: paged.attend(q.float(), k, v, table, lengths), "same 16-bit type")
+    refused(lambda: paged.attend(q[0], k, v, table, lengths), r"q is a tensor \[rows, heads, dim\]")
+    refused(lambda: paged.attend(q.float(), k, v, table, lengths), "q is f16 or bf16")
     refused(lambda: paged.attend(q.bfloat16(), k, v, table, lengths), "same 16-bit type")
     refused(lambda: paged.attend(q, k, v[:3], table, lengths), "two tensors")
     refused(lambda: paged.attend(q, k, v, table, lengths, k_scale=2.0), "scales belong")
     refused(lambda: paged.attend(q, *pages(dim=128), table, lengths), "heads of 64, pages of 128")
+    refused(lambda: paged.attend(q, k, v, None, lengths), "table is not a tensor")
+    refused(lambda: paged.attend(q, k, v, table, lengths, window=1 << 40), "window is beyond 31 bits")
+    refused(lambda: paged.attend(q, k, v, table, lengths, scale="a"), "scale is not a number")
     refused(lambda: paged.attend(q, k, v, table.long(), lengths), "table is an int32")
     refused(lambda: paged.attend(q, k, v, table, i32(4)), "lengths is a contiguous int32")
     refused(lambda: paged.attend(q, k, v, i32(2, 3).t(), lengths), "contiguous rows")
@@ -112,6 +122,7 @@ class Call:
     def __init__(self, paged, name, struct_):
         from emmy_ptx import driver
         self.entry, self.struct = getattr(driver.library(), f"emb_paged_{name}"), struct_
+        self.entry.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
 
     def refused(self, fields, match):
         from emmy_ptx import driver
@@ -145,7 +156,7 @@ def attend_fields(cache=(), **kw):
     (dict(width=1 << 28), "table row"), (dict(window=-1), "window"), (dict(scale=float("inf")), "finite"), (dict(lengths=0), "null table or lengths"),
     (dict(q=A + 2), "aligned"), (dict(q0=100), "multiple of 16 bytes"), (dict(o0=0), "overlap"), (dict(o0=64, o1=64), "overlap")])
 def test_attend_entry_refuses(paged, change, match):
-    Call(paged, "attend", paged._ATTEND).refused(attend_fields(**change), match)
+    Call(paged, "attend", ATTEND).refused(attend_fields(**change), match)
 
 
 def store_fields(cache=(), **kw):
@@ -161,7 +172,7 @@ def store_fields(cache=(), **kw):
     (dict(qw=A + 2), "norm weight"), (dict(slots=0), "null slots"), (dict(positions=0), "positions"), (dict(k=0), "null"), (dict(v0=4), "multiple of 16"),
     (dict(o0=128), "q_out overlap"), (dict(cache=dict(ks0=0)), "cache overlap"), (dict(cache=dict(vs1=64, vs2=64)), "cache overlap")])
 def test_store_entry_refuses(paged, change, match):
-    Call(paged, "store", paged._STORE).refused(store_fields(**change), match)
+    Call(paged, "store", STORE).refused(store_fields(**change), match)
 
 
 def assign_fields(**kw):
@@ -176,7 +187,7 @@ def assign_fields(**kw):
     (dict(cached=0), "null pointer"), (dict(free=0), "null pointer"), (dict(slots=0), "null pointer"), (dict(ts=3), "overlap"),
     (dict(lengths=A), "may not be"), (dict(head_out=A), "may not be"), (dict(width=1 << 27), "2^31")])
 def test_assign_entry_refuses(paged, change, match):
-    Call(paged, "assign", paged._ASSIGN).refused(assign_fields(**change), match)
+    Call(paged, "assign", ASSIGN).refused(assign_fields(**change), match)
 
 
 def test_null_arguments_are_refused(paged):
@@ -184,4 +195,3 @@ def test_null_arguments_are_refused(paged):
     for name in ("assign", "store", "attend"):
         assert getattr(driver.library(), f"emb_paged_{name}")(None, None) == -2
         assert b"null arguments" in driver.library().emb_last_error()
-    assert ctypes.sizeof(ctypes.c_void_p) == 8
