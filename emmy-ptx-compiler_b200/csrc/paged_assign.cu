@@ -11,6 +11,8 @@
 
 namespace {
 
+using namespace emb::paged;
+
 constexpr int THREADS = 256;
 constexpr int ROWS = 1024;  // rows of the step per CTA
 
@@ -56,6 +58,7 @@ __global__ void __launch_bounds__(THREADS) paged_assign_kernel(const emb_paged_a
     __shared__ long long taken_all;
     __shared__ int refused_all;
     const int tid = threadIdx.x;
+    follow_on();
     const long long row0 = static_cast<long long>(blockIdx.x) * ROWS;
     const long long row1 = min(row0 + ROWS, static_cast<long long>(a.tokens));
     const long long head = min(max(*a.free_head, 0), a.free_count), room = a.free_count - head;
@@ -134,7 +137,6 @@ __global__ void __launch_bounds__(THREADS) paged_assign_kernel(const emb_paged_a
 }  // namespace
 
 extern "C" int emb_paged_assign(const emb_paged_assign_t* args, void* stream) {
-    using namespace emb::paged;
     if (!args) return refuse("paged_assign: null arguments");
     const emb_paged_assign_t& a = *args;
     if (static_cast<int64_t>(a.table_width) * a.page_size >= (1ll << 31)) return refuse("paged_assign: a table row of 2^31 tokens or more");
@@ -147,6 +149,5 @@ extern "C" int emb_paged_assign(const emb_paged_assign_t* args, void* stream) {
     if (a.lengths && (a.lengths == a.cached || a.lengths == a.fresh)) return refuse("paged_assign: lengths may not be cached or fresh");
     if (a.free_head_out == a.free_head) return refuse("paged_assign: free_head_out may not be free_head");
     const unsigned grid = a.tokens > ROWS ? (static_cast<unsigned>(a.tokens) + ROWS - 1) / ROWS : 1u;
-    paged_assign_kernel<<<grid, THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return launched("launch of paged_assign");
+    return launched("launch of paged_assign", launch(paged_assign_kernel, grid, THREADS, 0, static_cast<cudaStream_t>(stream), a));
 }

@@ -27,8 +27,7 @@ inline int refuse(const char* fmt, ...) {
     return emb_fail_text(EMB_E_ARGUMENT, text);
 }
 
-inline int launched(const char* what) {
-    const cudaError_t e = cudaGetLastError();
+inline int launched(const char* what, cudaError_t e) {
     if (e == cudaSuccess) return 0;
     char text[256];
     snprintf(text, sizeof text, "%s: %s", what, cudaGetErrorString(e));
@@ -71,6 +70,22 @@ inline int check_cache(const char* who, const emb_paged_cache_t& c, int q_dtype)
             return refuse("%s: a stride of the pages is not a multiple of 16 bytes below 2^32 elements", who);
     if (!(c.k_scale > 0.f) || !(c.v_scale > 0.f) || c.k_scale > 3.0e38f || c.v_scale > 3.0e38f) return refuse("%s: a cache scale is not a positive number", who);
     return 0;
+}
+
+// Every kernel here is launched as a programmatic dependent of the work before it in the stream: its CTAs may be placed
+// while that work drains, which hides the launch, and before its first access to memory it waits until that work is
+// complete and visible (follow_on); at the same time it lets its own successor do the same.
+template <class... P, class... A> inline cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, unsigned smem, cudaStream_t stream, A... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid), config.blockDim = dim3(block), config.dynamicSmemBytes = smem, config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute, config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+__device__ __forceinline__ void follow_on() {
+    asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
 }
 
 struct E4m3 {

@@ -17,6 +17,7 @@ constexpr int THREADS = 128;
 
 template <class T, class C, int LANES> __global__ void __launch_bounds__(THREADS) paged_store_kernel(const emb_paged_store_t a) {
     const int lane = threadIdx.x % LANES;
+    follow_on();
     const int all_heads = a.heads + 2 * a.cache.kv_heads;
     const long long rows = static_cast<long long>(a.tokens) * all_heads;
     const long long row = static_cast<long long>(blockIdx.x) * (THREADS / LANES) + threadIdx.x / LANES;
@@ -100,12 +101,8 @@ template <class T, class C> int run_dim(const emb_paged_store_t& a, cudaStream_t
     const int per_cta = THREADS / (a.cache.dim / 8);
     const long long grid = (rows + per_cta - 1) / per_cta;
     if (grid > 0x7fffffffll) return refuse("paged_store: %lld head rows in one call", rows);
-    switch (a.cache.dim) {
-        case 64: paged_store_kernel<T, C, 8><<<static_cast<unsigned>(grid), THREADS, 0, stream>>>(a); break;
-        case 128: paged_store_kernel<T, C, 16><<<static_cast<unsigned>(grid), THREADS, 0, stream>>>(a); break;
-        default: paged_store_kernel<T, C, 32><<<static_cast<unsigned>(grid), THREADS, 0, stream>>>(a); break;
-    }
-    return launched("launch of paged_store");
+    const auto kernel = a.cache.dim == 64 ? paged_store_kernel<T, C, 8> : a.cache.dim == 128 ? paged_store_kernel<T, C, 16> : paged_store_kernel<T, C, 32>;
+    return launched("launch of paged_store", launch(kernel, static_cast<unsigned>(grid), THREADS, 0, stream, a));
 }
 
 }  // namespace
