@@ -6,11 +6,15 @@
 // was summed is scaled by 2^(m - m'). Every key and value is read once for the heads / kv_heads query heads that share it,
 // so the bound is HBM: 2 dim bytes of cache per 2 * group * dim multiply-adds of each product.
 //
-// The group's query heads are the 16 rows (MT tiles of them) of mma.sync m16n8k16; tcgen05 would want 128 rows, and the
-// tensor work of 16 rows is a tenth of what the legacy path does in the time HBM needs for the bytes. A WARP owns KEYS
+// Products are mma.sync m16n8k16 with the KEYS as rows: S^T = K Q^T (16 keys x 8 query heads) and O^T = V^T P^T (16 dims x
+// 8 heads), so a group of up to eight heads wastes no row, and S^T becomes the operand P^T by one 8 x 8 transposition
+// (movmatrix). tcgen05 would want 128 rows of one request and head at a time in shared memory as it lays them out; the
+// tensor work here is a tenth of what the legacy path does in the time HBM needs for the bytes. A WARP owns KEYS
 // consecutive keys at a time: it copies them into a ring of its own with cp.async (rows found through the page table, so any
 // page size and any strides; rows behind the length are filled with zeros and not read), multiplies, and keeps a maximum,
 // sum and output of its own. Warps meet only at the end of a request's head, so no barrier stands between copies and products.
+// The maximum that weights refer to moves only when a score passes it by more than 8 (a weight is at most 2^8, in f16 and f32
+// alike far from overflow): most steps then need neither the reduction over lanes nor the rescaling.
 //
 // The work is cut by TILES of WARPS * KEYS keys, all requests and heads behind one another: CTA c of n takes tiles
 // [c T / n, (c + 1) T / n), whatever their requests. So a single long request and a ragged batch both spread evenly, and
@@ -19,6 +23,7 @@
 
 #include "paged_common.cuh"
 
+#include <algorithm>
 #include <mutex>
 
 #include "emb_frag.cuh"
@@ -32,12 +37,15 @@ constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int WHOLE_TILES = 4;  // a request's head of at most so many tiles is not cut
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
-template <class T, class C, int DIM_, int MT_> struct Config {
-    static constexpr int DIM = DIM_, MT = MT_, ROWS = 16 * MT;
+constexpr float LOWEST = -3.402823466e38f;  // seed of a maximum: finite, so that a masked score (-inf) against it weighs 0
+constexpr float SLACK = 8.f;
+
+template <class T, class C, int DIM_, int HT_> struct Config {
+    static constexpr int DIM = DIM_, HT = HT_, ROWS = 8 * HT;  // query heads of a CTA, in tiles of eight
     static constexpr bool CODES = sizeof(C) == 1;
     static constexpr bool BF16 = !CODES && std::is_same<T, __nv_bfloat16>::value;  // type of the products
     static constexpr int ROW_BYTES = DIM * static_cast<int>(sizeof(C));
-    static constexpr int KEYS = ROW_BYTES <= 128 ? 32 : 16;  // of a warp per step
+    static constexpr int KEYS = ROW_BYTES <= 64 ? 64 : ROW_BYTES <= 128 ? 32 : 16;  // of a warp per step: 8 KB (16 KB at 512-byte rows)
     static constexpr int TILE = WARPS * KEYS;
     static constexpr int STEP_BYTES = 2 * KEYS * ROW_BYTES;  // keys, then values
     static constexpr int CTAS = DIM == 256 ? 1 : 2;  // per SM
@@ -45,7 +53,18 @@ template <class T, class C, int DIM_, int MT_> struct Config {
     static constexpr int PITCH = DIM + 4;  // floats of a row of a piece: outputs, maximum, sum
     static constexpr int MERGE_BYTES = WARPS * 8 * PITCH * 4;
     static constexpr int SMEM = WARPS * STAGES * STEP_BYTES + MERGE_BYTES;
-    static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
+    static_assert(CTAS * (SMEM + 1024 + 128) <= 228 * 1024, "shared memory of an SM");
+};
+
+// division by a number known to the host: floor(x / d) for x < 2^31
+struct Divisor {
+    uint32_t d, magic, shift;
+    explicit Divisor(uint32_t d_) : d(d_) {
+        shift = 0;
+        while ((1ull << shift) < d) ++shift;
+        magic = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t over(uint32_t x) const { return (__umulhi(x, magic) + x) >> shift; }
 };
 
 // where a piece's rows lie: the record of a CTA whose last head goes on in the next CTAs, and two pieces a CTA
@@ -129,10 +148,33 @@ __device__ __forceinline__ float exp2_(float x) {
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-template <class T, class C, int DIM, int MT>
-__global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, MT>::CTAS)) paged_attend_kernel(const emb_paged_attend_t a, Record* __restrict__ records, float* __restrict__ pieces) {
-    using Cfg = Config<T, C, DIM, MT>;
-    constexpr int KEYS = Cfg::KEYS, NT = KEYS / 8, DT = DIM / 8, ROW_BYTES = Cfg::ROW_BYTES, STAGES = Cfg::STAGES;
+// one more part of a row: its outputs and sum, scaled by f to the common maximum
+__device__ __forceinline__ void add_part(float4& acc, float& s, const float4& x, float f, float sum) {
+    acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+    s += f * sum;
+}
+
+// four dims of a finished row: rounded once; a row without keys is 0
+template <class Cfg, class T> __device__ __forceinline__ void put_out(const emb_paged_attend_t& a, int b, long long h, int d, const float4& acc, float best, float s) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    const float inv = s == 0.f ? 0.f : (Cfg::CODES ? a.cache.v_scale : 1.f) / s;
+    const uint2 packed = make_uint2(frag::pack_f32<BF16>(acc.x * inv, acc.y * inv), frag::pack_f32<BF16>(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[1] + d) = packed;
+    if (a.lse && d == 0) a.lse[b * static_cast<long long>(a.heads) + h] = s == 0.f ? -INFINITY : best * LN2 + logf(s);
+}
+
+// P^T of eight keys: from rows of keys (a lane: key g, heads 2 quad, 2 quad + 1) to the operand (keys 2 quad, 2 quad + 1, head g)
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <class T, class C, int DIM, int HT>
+__global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_attend_kernel(const emb_paged_attend_t a, const Divisor page_size, Record* __restrict__ records, float* __restrict__ pieces) {
+    using Cfg = Config<T, C, DIM, HT>;
+    constexpr int KEYS = Cfg::KEYS, KT = KEYS / 16, DT = DIM / 16, ROW_BYTES = Cfg::ROW_BYTES, STAGES = Cfg::STAGES;
+    constexpr int LOOKS = (KEYS + 31) / 32;  // keys that a lane looks up per step
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long scan_slab[WARPS], share[2];
     __shared__ long long first_before;  // tiles before the request that holds the share's first tile
@@ -176,6 +218,7 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, MT>::CTAS)) paged_
     if (tid < 2) share[tid] = all * (blockIdx.x + tid) / n;
     __syncthreads();
     const long long want0 = share[0], want1 = share[1];
+    __syncthreads();
     long long before_chunk = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
         if (a.requests > THREADS) {
@@ -203,42 +246,48 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, MT>::CTAS)) paged_
     ahead.head = static_cast<int>((x0 - first_before) / ahead.tiles);
     ahead.t = static_cast<uint32_t>((x0 - first_before) % ahead.tiles);
     Cursor now = ahead;
-    const bool first_is_cut = now.t > 0;  // the first head's tiles before these belong to an earlier CTA
 
     // ---- copies: a lane finds a key's row, the warp copies KEYS of them
     const uint32_t ring = frag::smem_addr(smem) + warp * (STAGES * Cfg::STEP_BYTES);
-    const uint32_t page_size = a.cache.page_size;
-    const bool pow2 = (page_size & (page_size - 1)) == 0;
-    const int page_shift = __ffs(page_size) - 1;
-    const auto token_of = [&]() { return ahead.span.begin + ahead.t * Cfg::TILE + warp * KEYS + (lane & (KEYS - 1)); };
-    const auto page_of = [&]() -> int {  // the page id of this lane's key, a step before it is needed
-        const uint32_t token = token_of();
-        if (ahead.b >= a.requests || token >= ahead.span.end) return 0;
-        const uint32_t index = pow2 ? token >> page_shift : token / page_size;
-        return index < static_cast<uint32_t>(a.table_width) ? __ldg(a.table + ahead.b * a.table_stride + index) : -1;
+    const bool same = a.cache.k_stride[0] == a.cache.v_stride[0] && a.cache.k_stride[1] == a.cache.v_stride[1] && a.cache.k_stride[2] == a.cache.v_stride[2];
+    const auto token_of = [&](int look) { return ahead.span.begin + ahead.t * Cfg::TILE + warp * KEYS + look * 32 + (lane & (KEYS < 32 ? KEYS - 1 : 31)); };
+    int page[LOOKS];  // ids of the pages of this lane's keys, loaded a step before they are needed
+    const auto find_pages = [&]() {
+#pragma unroll
+        for (int l = 0; l < LOOKS; ++l) {
+            const uint32_t token = token_of(l), index = page_size.over(token);
+            page[l] = -1;
+            if (token < ahead.span.end && index < static_cast<uint32_t>(a.table_width)) page[l] = __ldg(a.table + ahead.b * a.table_stride + index);
+        }
     };
-    const auto issue = [&](int stage, int page) {
-        const uint32_t token = token_of();
-        const uint32_t in_page = pow2 ? token & (page_size - 1) : token % page_size;
+    const auto issue = [&](int stage) {
         const int kv = ahead.head / heads.groups;
         // (-1: behind the length, zeros; -2: no such page, NaN)
-        long long k_at = -1, v_at = -1;
-        if (token < ahead.span.end) {
-            const bool known = page >= 0 && page < a.cache.pages;
-            k_at = known ? (page * a.cache.k_stride[0] + in_page * a.cache.k_stride[1] + kv * a.cache.k_stride[2]) * static_cast<int>(sizeof(C)) : -2;
-            v_at = known ? (page * a.cache.v_stride[0] + in_page * a.cache.v_stride[1] + kv * a.cache.v_stride[2]) * static_cast<int>(sizeof(C)) : -2;
+        long long k_at[LOOKS], v_at[LOOKS];
+#pragma unroll
+        for (int l = 0; l < LOOKS; ++l) {
+            const uint32_t token = token_of(l), in_page = token - page_size.over(token) * page_size.d;
+            k_at[l] = v_at[l] = -1;
+            if (token < ahead.span.end) {
+                const bool known = page[l] >= 0 && page[l] < a.cache.pages;
+                k_at[l] = known ? (page[l] * a.cache.k_stride[0] + in_page * a.cache.k_stride[1] + kv * a.cache.k_stride[2]) * static_cast<int>(sizeof(C)) : -2;
+                if (!same) v_at[l] = known ? (page[l] * a.cache.v_stride[0] + in_page * a.cache.v_stride[1] + kv * a.cache.v_stride[2]) * static_cast<int>(sizeof(C)) : -2;
+            }
         }
         constexpr int CHUNKS = ROW_BYTES / 16, PER_PASS = 32 / CHUNKS;
         const uint32_t to = ring + stage * Cfg::STEP_BYTES;
         const int chunk = lane % CHUNKS;
+        const char* const k_from = static_cast<const char*>(a.cache.k) + chunk * 16;
+        const char* const v_from = static_cast<const char*>(a.cache.v) + chunk * 16;
 #pragma unroll
         for (int p = 0; p < KEYS / PER_PASS; ++p) {
             const int row = p * PER_PASS + lane / CHUNKS;
-            const long long k_row = __shfl_sync(0xffffffffu, k_at, row), v_row = __shfl_sync(0xffffffffu, v_at, row);
+            const long long k_row = __shfl_sync(0xffffffffu, k_at[p * PER_PASS / 32], row & 31);
+            const long long v_row = same ? k_row : __shfl_sync(0xffffffffu, v_at[p * PER_PASS / 32], row & 31);
             const uint32_t k_to = to + place<ROW_BYTES>(row, chunk), v_to = k_to + KEYS * ROW_BYTES;
             if (k_row >= 0) {
-                copy16<ROW_BYTES>(k_to, static_cast<const char*>(a.cache.k) + k_row + chunk * 16);
-                copy16<ROW_BYTES>(v_to, static_cast<const char*>(a.cache.v) + v_row + chunk * 16);
+                copy16<ROW_BYTES>(k_to, k_from + k_row);
+                copy16<ROW_BYTES>(v_to, v_from + v_row);
             } else {
                 fill16(k_to, k_row == -1 ? 0u : Cfg::CODES ? 0x7f7f7f7fu : 0x7fff7fffu);
                 fill16(v_to, 0u);
@@ -247,141 +296,129 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, MT>::CTAS)) paged_
     };
 
     const long long steps = x1 - x0;
-    int page = page_of();
     long long issued = 0;
+    find_pages();
     const auto feed = [&](int stage) {
         if (issued < steps) {
-            issue(stage, page);
+            issue(stage);
             advance<Cfg>(ahead, a, heads.cut);
-            page = issued + 1 < steps ? page_of() : 0;
+            if (issued + 1 < steps) find_pages();
         }
         ++issued;
         frag::cp_async_commit();
     };
     for (int s = 0; s < STAGES - 1; ++s) feed(s);
 
-    uint32_t q[MT][DIM / 16][4];
-    float factor[MT][2];  // of a row's products: into score log2(e)
-    float top[MT][2], total[MT][2], o[MT][DT][4];
+    uint32_t q[HT][DT][2];
+    float factor[HT][2];                  // of the products of heads 2 quad and 2 quad + 1: into score log2(e)
+    float top[HT][2], total[HT][2];       // what their weights refer to; this lane's keys' part of the sum
+    float o[HT][DT][4];                   // dims g and g + 8 of 16 (codes: 2 g and 2 g + 1), heads 2 quad and 2 quad + 1
     const float scale = a.scale * LOG2E * (Cfg::CODES ? a.cache.k_scale : 1.f);
     const auto begin_head = [&]() {
         const int kv = now.head / heads.groups, row0 = (now.head % heads.groups) * Cfg::ROWS;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < HT; ++m) {
+            const int row = row0 + m * 8 + g;
+            const T* from = static_cast<const T*>(a.q) + now.b * a.q_stride[0] + (static_cast<long long>(kv) * heads.group + row) * a.q_stride[1];
+            const bool real = row < heads.group;
+            float mine = scale;
+            if (!Cfg::CODES) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int row = row0 + m * 16 + half * 8 + g;
-                const T* from = static_cast<const T*>(a.q) + now.b * a.q_stride[0] + (static_cast<long long>(kv) * heads.group + row) * a.q_stride[1];
-                const bool real = row < heads.group;
-                factor[m][half] = scale;
-                top[m][half] = -INFINITY, total[m][half] = 0.f;
-                if (!Cfg::CODES) {
+                for (int d = 0; d < DT; ++d) {
+                    q[m][d][0] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + quad * 2) : 0u;
+                    q[m][d][1] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + 8 + quad * 2) : 0u;
+                }
+            } else {
+                // an e4m3 row's dims 4 quad .. 4 quad + 3 come in one word, so the query's dims are dealt the same way. The
+                // product is of f16: a bf16 query's row is first scaled by a power of two to 1 <= max < 2, so that it fits
+                // (what falls below 2^-24 of the row's maximum is rounded away, far below the query's own 2^-8 steps)
+                uint2 raw[DT];
+                float most = 0.f;
 #pragma unroll
-                    for (int d = 0; d < DIM / 16; ++d) {
-                        q[m][d][half] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + quad * 2) : 0u;
-                        q[m][d][half + 2] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + 8 + quad * 2) : 0u;
-                    }
-                } else {
-                    // an e4m3 row's dims 4 quad .. 4 quad + 3 come in one word, so the query's dims are dealt the same way. The
-                    // product is of f16: a bf16 query's row is first scaled by a power of two to 1 <= max < 2, so that it fits
-                    // (what falls below 2^-24 of the row's maximum is rounded away, far below the query's own 2^-8 steps)
-                    uint2 raw[DIM / 16];
-                    float most = 0.f;
+                for (int d = 0; d < DT; ++d) {
+                    raw[d] = real ? *reinterpret_cast<const uint2*>(from + d * 16 + quad * 4) : make_uint2(0u, 0u);
+                    const T* x = reinterpret_cast<const T*>(&raw[d]);
 #pragma unroll
-                    for (int d = 0; d < DIM / 16; ++d) {
-                        raw[d] = real ? *reinterpret_cast<const uint2*>(from + d * 16 + quad * 4) : make_uint2(0u, 0u);
-                        const T* x = reinterpret_cast<const T*>(&raw[d]);
+                    for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(to_f32(x[e])));
+                }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                int power = ((__float_as_int(most) >> 23) & 255) - 127;
+                power = std::is_same<T, __half>::value ? 0 : max(-100, min(power, 120));
+                const float down = __int_as_float((127 - power) << 23);
+                mine = scale * __int_as_float((127 + power) << 23);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(to_f32(x[e])));
-                    }
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    int power = ((__float_as_int(most) >> 23) & 255) - 127;
-                    power = std::is_same<T, __half>::value ? 0 : max(-100, min(power, 120));
-                    const float down = __int_as_float((127 - power) << 23);
-                    factor[m][half] = scale * __int_as_float((127 + power) << 23);
-#pragma unroll
-                    for (int d = 0; d < DIM / 16; ++d) {
-                        const T* x = reinterpret_cast<const T*>(&raw[d]);
-                        q[m][d][half] = frag::pack_f32<false>(to_f32(x[0]) * down, to_f32(x[1]) * down);
-                        q[m][d][half + 2] = frag::pack_f32<false>(to_f32(x[2]) * down, to_f32(x[3]) * down);
-                    }
+                for (int d = 0; d < DT; ++d) {
+                    const T* x = reinterpret_cast<const T*>(&raw[d]);
+                    q[m][d][0] = frag::pack_f32<false>(to_f32(x[0]) * down, to_f32(x[1]) * down);
+                    q[m][d][1] = frag::pack_f32<false>(to_f32(x[2]) * down, to_f32(x[3]) * down);
                 }
             }
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int e = 0; e < 2; ++e) {
+                factor[m][e] = Cfg::CODES ? __shfl_sync(0xffffffffu, mine, (quad * 2 + e) * 4) : scale;
+                top[m][e] = LOWEST, total[m][e] = 0.f;
+            }
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[m][d][e] = 0.f;
+        }
     };
 
     float* const merge = reinterpret_cast<float*>(smem + WARPS * STAGES * Cfg::STEP_BYTES);
-    // the warps' maxima, sums and outputs of a head become one, eight rows at a time; whole heads go out, cut ones to a piece
+    // the warps' maxima, sums and outputs of a head become one, eight query heads at a time; whole heads go out, cut ones to a piece
     const auto end_head = [&](float* piece) {
         const int kv = now.head / heads.groups, row0 = (now.head % heads.groups) * Cfg::ROWS;
         const int rows = min(Cfg::ROWS, heads.group - row0);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < HT; ++m) {
+            if (m * 8 >= rows) break;
+            float sum[2] = {total[m][0], total[m][1]};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int base = m * 16 + half * 8;
-                if (base >= rows) break;
-                float sum = total[m][half];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                __syncthreads();  // the last eight rows are read
-                if (base + g < rows) {
-                    float* to = merge + (warp * 8 + g) * Cfg::PITCH;
+            for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        if (Cfg::CODES) {  // tiles 2d and 2d + 1 hold the even and odd dims of 16
-                            if (d % 2 == 0)
-                                *reinterpret_cast<float4*>(to + d * 8 + quad * 4) = make_float4(o[m][d][half * 2], o[m][d + 1 < DT ? d + 1 : d][half * 2], o[m][d][half * 2 + 1], o[m][d + 1 < DT ? d + 1 : d][half * 2 + 1]);
-                        } else {
-                            *reinterpret_cast<float2*>(to + d * 8 + quad * 2) = make_float2(o[m][d][half * 2], o[m][d][half * 2 + 1]);
-                        }
-                    }
-                    if (quad == 0) to[DIM] = top[m][half], to[DIM + 1] = sum;
+                for (int e = 0; e < 2; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
+            __syncthreads();  // the last eight heads are read
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (m * 8 + quad * 2 + e >= rows) continue;
+                float* to = merge + (warp * 8 + quad * 2 + e) * Cfg::PITCH;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    if (Cfg::CODES) *reinterpret_cast<float2*>(to + d * 16 + g * 2) = make_float2(o[m][d][e], o[m][d][e + 2]);
+                    else to[d * 16 + g] = o[m][d][e], to[d * 16 + g + 8] = o[m][d][e + 2];
                 }
-                __syncthreads();
-                for (int i = tid; i < 8 * (DIM / 4); i += THREADS) {
-                    const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
-                    if (base + r >= rows) break;
-                    float best = -INFINITY;
+                if (g == 0) to[DIM] = top[m][e], to[DIM + 1] = sum[e];
+            }
+            __syncthreads();
+            for (int i = tid; i < 8 * (DIM / 4); i += THREADS) {
+                const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
+                if (m * 8 + r >= rows) break;
+                float best = LOWEST;
 #pragma unroll
-                    for (int w = 0; w < WARPS; ++w) best = fmaxf(best, merge[(w * 8 + r) * Cfg::PITCH + DIM]);
-                    const float ref = best == -INFINITY ? 0.f : best;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    float s = 0.f;
+                for (int w = 0; w < WARPS; ++w) best = fmaxf(best, merge[(w * 8 + r) * Cfg::PITCH + DIM]);
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                float s = 0.f;
 #pragma unroll
-                    for (int w = 0; w < WARPS; ++w) {
-                        const float* from = merge + (w * 8 + r) * Cfg::PITCH;
-                        const float f = exp2_(from[DIM] - ref);
-                        const float4 x = *reinterpret_cast<const float4*>(from + d);
-                        acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-                        s += f * from[DIM + 1];
-                    }
-                    if (piece) {
-                        float* to = piece + (base + r) * Cfg::PITCH;
-                        *reinterpret_cast<float4*>(to + d) = acc;
-                        if (d == 0) to[DIM] = best, to[DIM + 1] = s;
-                    } else {
-                        const float inv = s == 0.f ? 0.f : (Cfg::CODES ? a.cache.v_scale : 1.f) / s;
-                        const long long h = static_cast<long long>(kv) * heads.group + row0 + base + r;
-                        uint2 packed;
-                        packed.x = frag::pack_f32<std::is_same<T, __nv_bfloat16>::value>(acc.x * inv, acc.y * inv);
-                        packed.y = frag::pack_f32<std::is_same<T, __nv_bfloat16>::value>(acc.z * inv, acc.w * inv);
-                        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + now.b * a.out_stride[0] + h * a.out_stride[1] + d) = packed;
-                        if (a.lse && d == 0) a.lse[now.b * static_cast<long long>(a.heads) + h] = s == 0.f ? -INFINITY : best * LN2 + logf(s);
-                    }
+                for (int w = 0; w < WARPS; ++w) {
+                    const float* from = merge + (w * 8 + r) * Cfg::PITCH;
+                    add_part(acc, s, *reinterpret_cast<const float4*>(from + d), exp2_(from[DIM] - best), from[DIM + 1]);
+                }
+                if (piece) {
+                    float* to = piece + (m * 8 + r) * Cfg::PITCH;
+                    *reinterpret_cast<float4*>(to + d) = acc;
+                    if (d == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(best, s);
+                } else {
+                    put_out<Cfg, T>(a, now.b, static_cast<long long>(kv) * heads.group + row0 + m * 8 + r, d, acc, best, s);
                 }
             }
+        }
     };
 
     begin_head();
     int stage = 0;
-    bool cut_in_front = first_is_cut;
+    bool cut_in_front = now.t > 0;  // the head's tiles before these belong to an earlier CTA
     Record record{0, 0, 0, 0};
     for (long long step = 0; step < steps; ++step) {
         frag::cp_async_wait<STAGES - 2>();
@@ -389,121 +426,117 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, MT>::CTAS)) paged_
         feed(stage == 0 ? STAGES - 1 : stage - 1);
         const uint32_t from = ring + stage * Cfg::STEP_BYTES;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
-
-        // ---- scores
-        float s[MT][NT][4];
+        const uint32_t token0 = now.span.begin + now.t * Cfg::TILE + warp * KEYS;
+        if (token0 < now.span.end) {
+            // ---- scores
+            float s[HT][KT][4];  // keys g and g + 8 of 16, heads 2 quad and 2 quad + 1
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < HT; ++m)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+                for (int j = 0; j < KT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[m][j][e] = 0.f;
+                    for (int e = 0; e < 4; ++e) s[m][j][e] = 0.f;
 #pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-            const int row = j * 16 + (lane & 7) + ((lane & 16) >> 1), chunk = (lane >> 3) & 1;
-            if (!Cfg::CODES) {
+            for (int j = 0; j < KT; ++j) {
+                if (!Cfg::CODES) {
 #pragma unroll
-                for (int d = 0; d < DIM / 16; ++d) {
-                    uint32_t r[4];
-                    load4(r, from + place<ROW_BYTES>(row, d * 2 + chunk));
+                    for (int d = 0; d < DT; ++d) {
+                        uint32_t r[4];
+                        load4(r, from + place<ROW_BYTES>(j * 16 + (lane & 15), d * 2 + (lane >> 4)));
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        frag::mma_f32<Cfg::BF16>(s[m][2 * j], q[m][d], reinterpret_cast<const uint32_t(&)[2]>(r[0]));
-                        frag::mma_f32<Cfg::BF16>(s[m][2 * j + 1], q[m][d], reinterpret_cast<const uint32_t(&)[2]>(r[2]));
+                        for (int m = 0; m < HT; ++m) frag::mma_f32<Cfg::BF16>(s[m][j], r, q[m][d]);
                     }
-                }
-            } else {
+                } else {
 #pragma unroll
-                for (int d = 0; d < DIM / 16; d += 2) {
-                    uint32_t r[4];
-                    load4(r, from + place<ROW_BYTES>(row, d + chunk));
+                    for (int d = 0; d < DT; d += 2) {
+                        uint32_t r[4];
+                        load4(r, from + place<ROW_BYTES>(j * 16 + (lane & 15), d + (lane >> 4)));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t w[2];
-                        widen4(r[i], w[0], w[1]);
+                        for (int i = 0; i < 2; ++i) {
+                            uint32_t w[4];
+                            widen4(r[2 * i], w[0], w[2]);
+                            widen4(r[2 * i + 1], w[1], w[3]);
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) frag::mma_f32<false>(s[m][2 * j + i / 2], q[m][d + i % 2], w);
+                            for (int m = 0; m < HT; ++m) frag::mma_f32<false>(s[m][j], w, q[m][d + i]);
+                        }
                     }
                 }
             }
-        }
 
-        // ---- softmax
-        const uint32_t token0 = now.span.begin + now.t * Cfg::TILE + warp * KEYS;
-        const bool ragged = token0 + KEYS > now.span.end;
-        uint32_t p[MT][NT / 2][4];
-        bool moved = false;
-        float keep[MT][2];
+            // ---- softmax
+            const bool ragged = token0 + KEYS > now.span.end;
+            float most[HT][2];
+            bool passed = false;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < HT; ++m)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float most = top[m][half];
+                for (int e = 0; e < 2; ++e) {
+                    most[m][e] = LOWEST;
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+                    for (int j = 0; j < KT; ++j)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            float& x = s[m][j][half * 2 + e];
+                            x *= factor[m][e];
+                            if (ragged && token0 + j * 16 + half * 8 + g >= now.span.end) x = -INFINITY;
+                            most[m][e] = fmaxf(most[m][e], x);
+                        }
+                    passed |= most[m][e] > top[m][e] + SLACK;
+                }
+            if (__any_sync(0xffffffffu, passed)) {
+#pragma unroll
+                for (int m = 0; m < HT; ++m)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float& x = s[m][j][half * 2 + e];
-                        x *= factor[m][half];
-                        if (ragged && token0 + j * 8 + quad * 2 + e >= now.span.end) x = -INFINITY;
-                        most = fmaxf(most, x);
-                    }
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const float ref = most == -INFINITY ? 0.f : most;
-                keep[m][half] = exp2_(top[m][half] - ref);
-                moved |= top[m][half] != most;
-                top[m][half] = most;
-                float sum = 0.f;
+                        float x = most[m][e];
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const float u = exp2_(s[m][j][half * 2] - ref), v = exp2_(s[m][j][half * 2 + 1] - ref);
-                    sum += u + v;
-                    // the weights' one rounding: the product with the values takes 16-bit operands (f16 or bf16)
-                    p[m][j / 2][half + (j % 2) * 2] = frag::pack_f32<Cfg::BF16>(u, v);
-                }
-                total[m][half] = total[m][half] * keep[m][half] + sum;
+                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        const float raised = fmaxf(top[m][e], x), keep = exp2_(top[m][e] - raised);
+                        top[m][e] = raised;
+                        total[m][e] *= keep;
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) o[m][d][e] *= keep, o[m][d][e + 2] *= keep;
+                    }
             }
-        if (__any_sync(0xffffffffu, moved)) {
+            uint32_t p[HT][KT][2];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < HT; ++m)
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
+                for (int j = 0; j < KT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[m][d][e] *= keep[m][e / 2];
-        }
-
-        // ---- values
-#pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-            const int row = j * 16 + (lane & 15), chunk = lane >> 4;
-            const uint32_t values = from + KEYS * ROW_BYTES;
-            if (!Cfg::CODES) {
-#pragma unroll
-                for (int d = 0; d < DT; d += 2) {
-                    uint32_t r[4];
-                    load4_trans(r, values + place<ROW_BYTES>(row, d + chunk));
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        frag::mma_f32<Cfg::BF16>(o[m][d], p[m][j], reinterpret_cast<const uint32_t(&)[2]>(r[0]));
-                        frag::mma_f32<Cfg::BF16>(o[m][d + 1], p[m][j], reinterpret_cast<const uint32_t(&)[2]>(r[2]));
+                    for (int half = 0; half < 2; ++half) {
+                        const float u = exp2_(s[m][j][half * 2] - top[m][0]), v = exp2_(s[m][j][half * 2 + 1] - top[m][1]);
+                        total[m][0] += u, total[m][1] += v;
+                        // the weights' one rounding: the product with the values takes 16-bit operands (f16 or bf16)
+                        p[m][j][half] = transposed(frag::pack_f32<Cfg::BF16>(u, v));
                     }
-                }
-            } else {
+
+            // ---- values
+            const uint32_t values = from + KEYS * ROW_BYTES;
 #pragma unroll
-                for (int d = 0; d < DT; d += 4) {  // 32 dims: two chunks of a row
-                    uint32_t r[4];
-                    load4_trans(r, values + place<ROW_BYTES>(row, d / 2 + chunk));
+            for (int j = 0; j < KT; ++j) {
+                const int row = j * 16 + (lane & 7) + ((lane & 16) >> 1), chunk = (lane >> 3) & 1;
+                if (!Cfg::CODES) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        // a word holds dims (2g, 2g + 1) of two keys: sorted by dim, the even dims make one tile and the odd another
-                        uint32_t even[2], odd[2];
-                        widen4(__byte_perm(r[2 * c], 0, 0x3120), even[0], odd[0]);
-                        widen4(__byte_perm(r[2 * c + 1], 0, 0x3120), even[1], odd[1]);
+                    for (int d = 0; d < DT; ++d) {
+                        uint32_t r[4];
+                        load4_trans(r, values + place<ROW_BYTES>(row, d * 2 + chunk));
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            frag::mma_f32<false>(o[m][d + 2 * c], p[m][j], even);
-                            frag::mma_f32<false>(o[m][d + 2 * c + 1], p[m][j], odd);
+                        for (int m = 0; m < HT; ++m) frag::mma_f32<Cfg::BF16>(o[m][d], r, p[m][j]);
+                    }
+                } else {
+#pragma unroll
+                    for (int d = 0; d < DT; d += 2) {
+                        uint32_t r[4];
+                        load4_trans(r, values + place<ROW_BYTES>(row, d + chunk));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            // a word holds dims (2g, 2g + 1) of two keys: sorted by dim, the even dims are the tile's first eight rows
+                            uint32_t w[4];
+                            widen4(__byte_perm(r[i], 0, 0x3120), w[0], w[1]);
+                            widen4(__byte_perm(r[i + 2], 0, 0x3120), w[2], w[3]);
+#pragma unroll
+                            for (int m = 0; m < HT; ++m) frag::mma_f32<false>(o[m][d + i], w, p[m][j]);
                         }
                     }
                 }
@@ -529,41 +562,56 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, MT>::CTAS)) paged_
 }
 
 // The pieces of the heads that were cut: CTA c adds up those of the head that starts in CTA c's share and goes on. A row's
-// maximum and sum are joined as in the kernel above, always in the keys' order, so results do not depend on timing.
-template <class T, class C, int DIM, int MT>
-__global__ void __launch_bounds__(128) paged_join_kernel(const emb_paged_attend_t a, const Record* records, const float* pieces) {
-    using Cfg = Config<T, C, DIM, MT>;
+// maximum and sum are joined as in the kernel above. A row's pieces are dealt to JOIN_SPLIT warps, whose parts are added in
+// order: always the same order, so results do not depend on timing.
+constexpr int JOIN_WARPS = 8, JOIN_ROWS = 4, JOIN_SPLIT = JOIN_WARPS / JOIN_ROWS;
+
+template <class T, class C, int DIM, int HT>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_paged_attend_t a, const Record* records, const float* pieces) {
+    using Cfg = Config<T, C, DIM, HT>;
+    constexpr int PER_LANE = DIM / 32;  // dims of a lane: two of DIM 64, else fours
+    __shared__ float slab[JOIN_WARPS][Cfg::PITCH];
     follow_on();
     const Record record = records[blockIdx.x];
     if (record.pieces == 0) return;
     const Heads heads(a, Cfg::ROWS);
     const int kv = record.head / heads.groups, row0 = (record.head % heads.groups) * Cfg::ROWS;
     const int rows = min(Cfg::ROWS, heads.group - row0);
-    const auto piece_of = [&](int i, int row) {
-        return pieces + (2ll * (blockIdx.x + i) + (i == 0)) * (Cfg::ROWS * Cfg::PITCH) + row * Cfg::PITCH;
-    };
-    for (int i = threadIdx.x; i < rows * (DIM / 4); i += blockDim.x) {
-        const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
-        float best = -INFINITY;
-        for (int k = 0; k < record.pieces; ++k) best = fmaxf(best, piece_of(k, r)[DIM]);
-        const float ref = best == -INFINITY ? 0.f : best;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float s = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < record.pieces; ++k) {
-            const float* from = piece_of(k, r);
-            const float f = exp2_(from[DIM] - ref);
-            const float4 x = *reinterpret_cast<const float4*>(from + d);
-            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-            s += f * from[DIM + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % JOIN_SPLIT;
+    for (int base = blockIdx.y * JOIN_ROWS; base < rows; base += gridDim.y * JOIN_ROWS) {
+        const int r = min(base + warp / JOIN_SPLIT, rows - 1);
+        const auto piece_of = [&](int i) { return pieces + (2ll * (blockIdx.x + i) + (i == 0)) * (Cfg::ROWS * Cfg::PITCH) + r * Cfg::PITCH; };
+        float best = LOWEST;
+        for (int k = lane; k < record.pieces; k += 32) best = fmaxf(best, piece_of(k)[DIM]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+        float acc[PER_LANE] = {}, s = 0.f;
+#pragma unroll 8
+        for (int k = part; k < record.pieces; k += JOIN_SPLIT) {
+            const float* from = piece_of(k);
+            const float2 stat = *reinterpret_cast<const float2*>(from + DIM);
+            const float f = exp2_(stat.x - best);
+#pragma unroll
+            for (int e = 0; e < PER_LANE; ++e) acc[e] += f * from[e * 32 + lane];
+            s += f * stat.y;
         }
-        const float inv = s == 0.f ? 0.f : (Cfg::CODES ? a.cache.v_scale : 1.f) / s;
-        const long long h = static_cast<long long>(kv) * heads.group + row0 + r;
-        uint2 packed;
-        packed.x = frag::pack_f32<std::is_same<T, __nv_bfloat16>::value>(acc.x * inv, acc.y * inv);
-        packed.y = frag::pack_f32<std::is_same<T, __nv_bfloat16>::value>(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + record.request * a.out_stride[0] + h * a.out_stride[1] + d) = packed;
-        if (a.lse && d == 0) a.lse[record.request * static_cast<long long>(a.heads) + h] = s == 0.f ? -INFINITY : best * LN2 + logf(s);
+        __syncthreads();  // the last rows' parts are read
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) slab[warp][e * 32 + lane] = acc[e];
+        if (lane == 0) slab[warp][DIM] = s;
+        __syncthreads();
+        if (part == 0 && base + warp / JOIN_SPLIT < rows) {
+            s = 0.f;
+#pragma unroll
+            for (int w = 0; w < JOIN_SPLIT; ++w) s += slab[warp + w][DIM];
+            for (int d = lane * 4; d < DIM; d += 128) {
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                float none = 0.f;
+#pragma unroll
+                for (int w = 0; w < JOIN_SPLIT; ++w) add_part(sum, none, *reinterpret_cast<const float4*>(&slab[warp + w][d]), 1.f, 0.f);
+                put_out<Cfg, T>(a, record.request, static_cast<long long>(kv) * heads.group + row0 + r, d, sum, best, s);
+            }
+        }
     }
 }
 
@@ -584,16 +632,21 @@ int sm_count() {
 
 template <class Cfg> int64_t piece_bytes() { return 2ll * Cfg::ROWS * Cfg::PITCH * 4; }
 
-// the CTAs of a launch: as many as the SMs hold at once
+// no request has more keys (one without a page among them where a length is beyond its table row)
+int64_t longest_of(const emb_paged_attend_t& a) {
+    const int64_t most = static_cast<int64_t>(a.table_width) * a.cache.page_size + 1;
+    return a.window ? std::min<int64_t>(a.window, most) : most;
+}
+
+// the CTAs of a launch: as many as the SMs hold at once, or as there can be tiles
 template <class Cfg> int grid_of(const emb_paged_attend_t& a, int sms) {
-    const int64_t longest = a.window ? min(static_cast<int64_t>(a.window), static_cast<int64_t>(a.table_width) * a.cache.page_size + 1) : static_cast<int64_t>(a.table_width) * a.cache.page_size + 1;
-    const double most = static_cast<double>(a.requests) * Heads(a, Cfg::ROWS).cut * ((longest + Cfg::TILE - 1) / Cfg::TILE);
+    const double most = static_cast<double>(a.requests) * Heads(a, Cfg::ROWS).cut * ((longest_of(a) + Cfg::TILE - 1) / Cfg::TILE);
     const int all = sms * Cfg::CTAS;
     return most < all ? static_cast<int>(most) : all;
 }
 
-template <class T, class C, int DIM, int MT> int run(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {
-    using Cfg = Config<T, C, DIM, MT>;
+template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {
+    using Cfg = Config<T, C, DIM, HT>;
     const int sms = sm_count();
     if (!sms) return refuse("paged_attend: the current device cannot be asked for its SMs");
     const int grid = grid_of<Cfg>(a, sms);
@@ -604,23 +657,26 @@ template <class T, class C, int DIM, int MT> int run(const emb_paged_attend_t& a
     }
     if (a.workspace_bytes < bytes || !a.workspace || !aligned16(a.workspace))
         return refuse("paged_attend: a workspace of %lld bytes (16-byte aligned) is needed, not %lld", static_cast<long long>(bytes), static_cast<long long>(a.workspace_bytes));
-    auto kernel = paged_attend_kernel<T, C, DIM, MT>;
+    auto kernel = paged_attend_kernel<T, C, DIM, HT>;
     static std::once_flag once[MAX_DEVICES];
     int device = 0;
     cudaGetDevice(&device);
     std::call_once(once[device], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM); });
     Record* records = static_cast<Record*>(a.workspace);
     float* pieces = reinterpret_cast<float*>(records + grid);
-    if (int r = launched("launch of paged_attend", launch(kernel, grid, THREADS, Cfg::SMEM, stream, a, records, pieces))) return r;
-    return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, MT>, grid, 128, 0, stream, a, records, pieces));
+    if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), records, pieces))) return r;
+    if (longest_of(a) <= WHOLE_TILES * Cfg::TILE) return 0;  // no head can have been cut
+    const int group = min(a.heads / a.cache.kv_heads, static_cast<int>(Cfg::ROWS));
+    const dim3 join_grid(grid, (group + JOIN_ROWS - 1) / JOIN_ROWS);
+    return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, HT>, join_grid, JOIN_WARPS * 32, 0, stream, a, records, pieces));
 }
 
 template <class T, class C> int run_dim(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {
-    const bool wide = a.heads / a.cache.kv_heads > 16;
+    const int group = a.heads / a.cache.kv_heads;
     switch (a.cache.dim) {
-        case 64: return wide ? run<T, C, 64, 2>(a, stream, need) : run<T, C, 64, 1>(a, stream, need);
-        case 128: return wide ? run<T, C, 128, 2>(a, stream, need) : run<T, C, 128, 1>(a, stream, need);
-        default: return run<T, C, 256, 1>(a, stream, need);
+        case 64: return group <= 8 ? run<T, C, 64, 1>(a, stream, need) : group <= 16 ? run<T, C, 64, 2>(a, stream, need) : run<T, C, 64, 4>(a, stream, need);
+        case 128: return group <= 8 ? run<T, C, 128, 1>(a, stream, need) : group <= 16 ? run<T, C, 128, 2>(a, stream, need) : run<T, C, 128, 4>(a, stream, need);
+        default: return group <= 8 ? run<T, C, 256, 1>(a, stream, need) : run<T, C, 256, 2>(a, stream, need);
     }
 }
 
@@ -630,7 +686,7 @@ int attend(const emb_paged_attend_t* args, void* stream, int64_t* need) {
     if (int r = check_cache("paged_attend", a.cache, a.dtype)) return r;
     if (a.requests < 0 || a.heads < 1 || a.heads > 65535 || a.heads % a.cache.kv_heads)
         return refuse("paged_attend: %d requests of %d heads over %d key heads: a multiple of the key heads", a.requests, a.heads, a.cache.kv_heads);
-    if (a.table_width < 1 || static_cast<int64_t>(a.table_width) * a.cache.page_size >= (1ll << 31) || a.table_stride < 0)
+    if (a.table_width < 1 || static_cast<int64_t>(a.table_width) * a.cache.page_size >= (1ll << 31) - 1024 || a.table_stride < 0)
         return refuse("paged_attend: a table row of %d pages of %d tokens", a.table_width, a.cache.page_size);
     if (a.window < 0) return refuse("paged_attend: a negative window");
     if (!(a.scale > -INFINITY && a.scale < INFINITY)) return refuse("paged_attend: the scale is not a finite number");

@@ -75,9 +75,9 @@ inline int check_cache(const char* who, const emb_paged_cache_t& c, int q_dtype)
 // Every kernel here is launched as a programmatic dependent of the work before it in the stream: its CTAs may be placed
 // while that work drains, which hides the launch, and before its first access to memory it waits until that work is
 // complete and visible (follow_on); at the same time it lets its own successor do the same.
-template <class... P, class... A> inline cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, unsigned smem, cudaStream_t stream, A... args) {
+template <class... P, class... A> inline cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned block, unsigned smem, cudaStream_t stream, A... args) {
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(grid), config.blockDim = dim3(block), config.dynamicSmemBytes = smem, config.stream = stream;
+    config.gridDim = grid, config.blockDim = dim3(block), config.dynamicSmemBytes = smem, config.stream = stream;
     cudaLaunchAttribute attribute = {};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
