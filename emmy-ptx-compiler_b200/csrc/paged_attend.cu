@@ -33,8 +33,9 @@ namespace {
 using namespace emb::paged;
 namespace frag = emb::frag;
 
-constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int WHOLE_TILES = 4;  // a request's head of at most so many tiles is not cut
+// Where there are no more tiles than CTAs, a request's head of at most so many tiles is not cut: on a machine that is not
+// full a CTA takes about half a microsecond for a tile more, and the join two.
+constexpr int WHOLE_TILES = 4;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 constexpr float LOWEST = -3.402823466e38f;  // seed of a maximum: finite, so that a masked score (-inf) against it weighs 0
@@ -45,14 +46,17 @@ template <class T, class C, int DIM_, int HT_> struct Config {
     static constexpr bool CODES = sizeof(C) == 1;
     static constexpr bool BF16 = !CODES && std::is_same<T, __nv_bfloat16>::value;  // type of the products
     static constexpr int ROW_BYTES = DIM * static_cast<int>(sizeof(C));
-    static constexpr int KEYS = ROW_BYTES <= 64 ? 64 : ROW_BYTES <= 128 ? 32 : 16;  // of a warp per step: 8 KB (16 KB at 512-byte rows)
+    static constexpr int KEYS = ROW_BYTES >= 256 || (ROW_BYTES == 128 && HT == 4) ? 16 : ROW_BYTES == 128 || HT == 4 ? 32 : 64;  // of a warp per step
+    static constexpr int STEP_BYTES = 2 * KEYS * ROW_BYTES;                         // keys, then values
+    static constexpr int WARPS = ROW_BYTES == 512 ? 3 : 4, THREADS = WARPS * 32;
+    static constexpr int CTAS = DIM * HT > 256 || ROW_BYTES == 512 ? 2 : 3;  // per SM
     static constexpr int TILE = WARPS * KEYS;
-    static constexpr int STEP_BYTES = 2 * KEYS * ROW_BYTES;  // keys, then values
-    static constexpr int CTAS = DIM == 256 ? 1 : 2;  // per SM
-    static constexpr int STAGES = (192 / CTAS) * 1024 / (WARPS * STEP_BYTES);
-    static constexpr int PITCH = DIM + 4;  // floats of a row of a piece: outputs, maximum, sum
-    static constexpr int MERGE_BYTES = WARPS * 8 * PITCH * 4;
+    static constexpr int PITCH = DIM + 4;         // floats of a row of a piece: outputs, maximum, sum
+    static constexpr int MERGED = 512 / DIM;      // query heads whose parts the warps merge at a time
+    static constexpr int MERGE_BYTES = WARPS * MERGED * PITCH * 4;
+    static constexpr int STAGES = (228 * 1024 / CTAS - 1024 - 128 - MERGE_BYTES) / (WARPS * STEP_BYTES);
     static constexpr int SMEM = WARPS * STAGES * STEP_BYTES + MERGE_BYTES;
+    static_assert(STAGES >= 2, "a step is copied while another is multiplied");
     static_assert(CTAS * (SMEM + 1024 + 128) <= 228 * 1024, "shared memory of an SM");
 };
 
@@ -171,9 +175,9 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 
 template <class T, class C, int DIM, int HT>
-__global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_attend_kernel(const emb_paged_attend_t a, const Divisor page_size, Record* __restrict__ records, float* __restrict__ pieces) {
+__global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C, DIM, HT>::CTAS)) paged_attend_kernel(const emb_paged_attend_t a, const Divisor page_size, Record* __restrict__ records, float* __restrict__ pieces) {
     using Cfg = Config<T, C, DIM, HT>;
-    constexpr int KEYS = Cfg::KEYS, KT = KEYS / 16, DT = DIM / 16, ROW_BYTES = Cfg::ROW_BYTES, STAGES = Cfg::STAGES;
+    constexpr int WARPS = Cfg::WARPS, THREADS = Cfg::THREADS, KEYS = Cfg::KEYS, KT = KEYS / 16, DT = DIM / 16, ROW_BYTES = Cfg::ROW_BYTES, STAGES = Cfg::STAGES;
     constexpr int LOOKS = (KEYS + 31) / 32;  // keys that a lane looks up per step
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long scan_slab[WARPS], share[2];
@@ -215,6 +219,7 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
         if (tid == 0) records[blockIdx.x].pieces = 0;
         return;
     }
+    const uint32_t whole = all <= static_cast<long long>(gridDim.x) ? WHOLE_TILES : 0;
     if (tid < 2) share[tid] = all * (blockIdx.x + tid) / n;
     __syncthreads();
     const long long want0 = share[0], want1 = share[1];
@@ -228,10 +233,10 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
         const long long from = upto - static_cast<long long>(tiles) * heads.cut;
         // a border inside a head that is not to be cut moves to the head's first tile
         if (from <= want0 && want0 < upto) {
-            const long long x = tiles <= WHOLE_TILES ? from + (want0 - from) / tiles * tiles : want0;
+            const long long x = tiles <= whole ? from + (want0 - from) / tiles * tiles : want0;
             share[0] = x, first_request = base + tid, first_before = from;
         }
-        if (from <= want1 && want1 < upto && tiles <= WHOLE_TILES) share[1] = from + (want1 - from) / tiles * tiles;
+        if (from <= want1 && want1 < upto && tiles <= whole) share[1] = from + (want1 - from) / tiles * tiles;
     }
     __syncthreads();
     const long long x0 = share[0], x1 = share[1];
@@ -249,46 +254,55 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
 
     // ---- copies: a lane finds a key's row, the warp copies KEYS of them
     const uint32_t ring = frag::smem_addr(smem) + warp * (STAGES * Cfg::STEP_BYTES);
-    const bool same = a.cache.k_stride[0] == a.cache.v_stride[0] && a.cache.k_stride[1] == a.cache.v_stride[1] && a.cache.k_stride[2] == a.cache.v_stride[2];
+    const uint32_t k_stride[3] = {static_cast<uint32_t>(a.cache.k_stride[0]), static_cast<uint32_t>(a.cache.k_stride[1]), static_cast<uint32_t>(a.cache.k_stride[2])};
+    const uint32_t v_stride[3] = {static_cast<uint32_t>(a.cache.v_stride[0]), static_cast<uint32_t>(a.cache.v_stride[1]), static_cast<uint32_t>(a.cache.v_stride[2])};
+    const bool same = k_stride[0] == v_stride[0] && k_stride[1] == v_stride[1] && k_stride[2] == v_stride[2];
     const auto token_of = [&](int look) { return ahead.span.begin + ahead.t * Cfg::TILE + warp * KEYS + look * 32 + (lane & (KEYS < 32 ? KEYS - 1 : 31)); };
-    int page[LOOKS];  // ids of the pages of this lane's keys, loaded a step before they are needed
+    // of this lane's keys, found a step before they are needed: the page id (-1: behind the length, -2: none) and the token in it
+    int page[LOOKS];
+    uint32_t in_page[LOOKS];
     const auto find_pages = [&]() {
 #pragma unroll
         for (int l = 0; l < LOOKS; ++l) {
             const uint32_t token = token_of(l), index = page_size.over(token);
+            in_page[l] = token - index * page_size.d;
             page[l] = -1;
-            if (token < ahead.span.end && index < static_cast<uint32_t>(a.table_width)) page[l] = __ldg(a.table + ahead.b * a.table_stride + index);
+            if (token < ahead.span.end) {
+                const uint32_t id = index < static_cast<uint32_t>(a.table_width) ? __ldg(a.table + ahead.b * a.table_stride + index) : -2;
+                page[l] = min(id, 0xfffffffeu);  // (an entry of -1 is a page that is not there, too)
+            }
         }
     };
     const auto issue = [&](int stage) {
-        const int kv = ahead.head / heads.groups;
-        // (-1: behind the length, zeros; -2: no such page, NaN)
+        const uint32_t kv = ahead.head / heads.groups;
+        // byte offsets of the keys' rows (strides are below 2^32 elements), or the page id where there is no row
         long long k_at[LOOKS], v_at[LOOKS];
+        bool known = true;
 #pragma unroll
         for (int l = 0; l < LOOKS; ++l) {
-            const uint32_t token = token_of(l), in_page = token - page_size.over(token) * page_size.d;
-            k_at[l] = v_at[l] = -1;
-            if (token < ahead.span.end) {
-                const bool known = page[l] >= 0 && page[l] < a.cache.pages;
-                k_at[l] = known ? (page[l] * a.cache.k_stride[0] + in_page * a.cache.k_stride[1] + kv * a.cache.k_stride[2]) * static_cast<int>(sizeof(C)) : -2;
-                if (!same) v_at[l] = known ? (page[l] * a.cache.v_stride[0] + in_page * a.cache.v_stride[1] + kv * a.cache.v_stride[2]) * static_cast<int>(sizeof(C)) : -2;
-            }
+            const bool one = static_cast<uint32_t>(page[l]) < static_cast<uint32_t>(a.cache.pages);
+            const unsigned long long id = static_cast<uint32_t>(page[l]);
+            k_at[l] = one ? (id * k_stride[0] + static_cast<unsigned long long>(in_page[l]) * k_stride[1] + static_cast<unsigned long long>(kv) * k_stride[2]) * sizeof(C) : page[l] == -1 ? -1 : -2;
+            v_at[l] = k_at[l];
+            if (!same && one) v_at[l] = (id * v_stride[0] + static_cast<unsigned long long>(in_page[l]) * v_stride[1] + static_cast<unsigned long long>(kv) * v_stride[2]) * sizeof(C);
+            known = known && one;
         }
         constexpr int CHUNKS = ROW_BYTES / 16, PER_PASS = 32 / CHUNKS;
         const uint32_t to = ring + stage * Cfg::STEP_BYTES;
         const int chunk = lane % CHUNKS;
         const char* const k_from = static_cast<const char*>(a.cache.k) + chunk * 16;
         const char* const v_from = static_cast<const char*>(a.cache.v) + chunk * 16;
+        const bool all_known = __all_sync(0xffffffffu, known);
 #pragma unroll
         for (int p = 0; p < KEYS / PER_PASS; ++p) {
             const int row = p * PER_PASS + lane / CHUNKS;
             const long long k_row = __shfl_sync(0xffffffffu, k_at[p * PER_PASS / 32], row & 31);
             const long long v_row = same ? k_row : __shfl_sync(0xffffffffu, v_at[p * PER_PASS / 32], row & 31);
             const uint32_t k_to = to + place<ROW_BYTES>(row, chunk), v_to = k_to + KEYS * ROW_BYTES;
-            if (k_row >= 0) {
+            if (all_known || k_row >= 0) {
                 copy16<ROW_BYTES>(k_to, k_from + k_row);
                 copy16<ROW_BYTES>(v_to, v_from + v_row);
-            } else {
+            } else {  // behind the length: zeros; no such page: keys of NaN
                 fill16(k_to, k_row == -1 ? 0u : Cfg::CODES ? 0x7f7f7f7fu : 0x7fff7fffu);
                 fill16(v_to, 0u);
             }
@@ -313,20 +327,23 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
     float factor[HT][2];                  // of the products of heads 2 quad and 2 quad + 1: into score log2(e)
     float top[HT][2], total[HT][2];       // what their weights refer to; this lane's keys' part of the sum
     float o[HT][DT][4];                   // dims g and g + 8 of 16 (codes: 2 g and 2 g + 1), heads 2 quad and 2 quad + 1
-    const float scale = a.scale * LOG2E * (Cfg::CODES ? a.cache.k_scale : 1.f);
+    // a negative scale turns the query's signs, and scale 0 is a query of 0: so the largest product is the largest score
+    // (and a scale that underflows stays above 0: a masked score is -inf and not -inf * 0)
+    const float scale = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * LOG2E * (Cfg::CODES ? a.cache.k_scale : 1.f), 1.2e-38f);
+    const uint32_t turn = a.scale < 0.f ? 0x80008000u : 0u;
     const auto begin_head = [&]() {
         const int kv = now.head / heads.groups, row0 = (now.head % heads.groups) * Cfg::ROWS;
 #pragma unroll
         for (int m = 0; m < HT; ++m) {
             const int row = row0 + m * 8 + g;
             const T* from = static_cast<const T*>(a.q) + now.b * a.q_stride[0] + (static_cast<long long>(kv) * heads.group + row) * a.q_stride[1];
-            const bool real = row < heads.group;
+            const bool real = row < heads.group && a.scale != 0.f;
             float mine = scale;
             if (!Cfg::CODES) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    q[m][d][0] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + quad * 2) : 0u;
-                    q[m][d][1] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + 8 + quad * 2) : 0u;
+                    q[m][d][0] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + quad * 2) ^ turn : 0u;
+                    q[m][d][1] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + 8 + quad * 2) ^ turn : 0u;
                 }
             } else {
                 // an e4m3 row's dims 4 quad .. 4 quad + 3 come in one word, so the query's dims are dealt the same way. The
@@ -346,12 +363,12 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
                 int power = ((__float_as_int(most) >> 23) & 255) - 127;
                 power = std::is_same<T, __half>::value ? 0 : max(-100, min(power, 120));
                 const float down = __int_as_float((127 - power) << 23);
-                mine = scale * __int_as_float((127 + power) << 23);
+                mine = fmaxf(scale * __int_as_float((127 + power) << 23), 1.2e-38f);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     const T* x = reinterpret_cast<const T*>(&raw[d]);
-                    q[m][d][0] = frag::pack_f32<false>(to_f32(x[0]) * down, to_f32(x[1]) * down);
-                    q[m][d][1] = frag::pack_f32<false>(to_f32(x[2]) * down, to_f32(x[3]) * down);
+                    q[m][d][0] = frag::pack_f32<false>(to_f32(x[0]) * down, to_f32(x[1]) * down) ^ turn;
+                    q[m][d][1] = frag::pack_f32<false>(to_f32(x[2]) * down, to_f32(x[3]) * down) ^ turn;
                 }
             }
 #pragma unroll
@@ -379,11 +396,15 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
             for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
-            __syncthreads();  // the last eight heads are read
+#pragma unroll
+            for (int first = 0; first < 8; first += Cfg::MERGED) {
+            if (m * 8 + first >= rows) break;
+            __syncthreads();  // the last heads are read
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                if (m * 8 + quad * 2 + e >= rows) continue;
-                float* to = merge + (warp * 8 + quad * 2 + e) * Cfg::PITCH;
+                const int r = quad * 2 + e - first;
+                if (r < 0 || r >= Cfg::MERGED || m * 8 + first + r >= rows) continue;
+                float* to = merge + (warp * Cfg::MERGED + r) * Cfg::PITCH;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     if (Cfg::CODES) *reinterpret_cast<float2*>(to + d * 16 + g * 2) = make_float2(o[m][d][e], o[m][d][e + 2]);
@@ -392,26 +413,27 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
                 if (g == 0) to[DIM] = top[m][e], to[DIM + 1] = sum[e];
             }
             __syncthreads();
-            for (int i = tid; i < 8 * (DIM / 4); i += THREADS) {
-                const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
-                if (m * 8 + r >= rows) break;
+            for (int i = tid; i < Cfg::MERGED * (DIM / 4); i += THREADS) {
+                const int r = i / (DIM / 4), d = i % (DIM / 4) * 4, row = m * 8 + first + r;
+                if (row >= rows) break;
                 float best = LOWEST;
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) best = fmaxf(best, merge[(w * 8 + r) * Cfg::PITCH + DIM]);
+                for (int w = 0; w < WARPS; ++w) best = fmaxf(best, merge[(w * Cfg::MERGED + r) * Cfg::PITCH + DIM]);
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
                 float s = 0.f;
 #pragma unroll
                 for (int w = 0; w < WARPS; ++w) {
-                    const float* from = merge + (w * 8 + r) * Cfg::PITCH;
+                    const float* from = merge + (w * Cfg::MERGED + r) * Cfg::PITCH;
                     add_part(acc, s, *reinterpret_cast<const float4*>(from + d), exp2_(from[DIM] - best), from[DIM + 1]);
                 }
                 if (piece) {
-                    float* to = piece + (m * 8 + r) * Cfg::PITCH;
+                    float* to = piece + row * Cfg::PITCH;
                     *reinterpret_cast<float4*>(to + d) = acc;
                     if (d == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(best, s);
                 } else {
-                    put_out<Cfg, T>(a, now.b, static_cast<long long>(kv) * heads.group + row0 + m * 8 + r, d, acc, best, s);
+                    put_out<Cfg, T>(a, now.b, static_cast<long long>(kv) * heads.group + row0 + row, d, acc, best, s);
                 }
+            }
             }
         }
     };
@@ -429,13 +451,14 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
         const uint32_t token0 = now.span.begin + now.t * Cfg::TILE + warp * KEYS;
         if (token0 < now.span.end) {
             // ---- scores
-            float s[HT][KT][4];  // keys g and g + 8 of 16, heads 2 quad and 2 quad + 1
+            constexpr int CHAINS = HT * KT >= 4 ? 1 : 2;  // sums that a score is made of: products of one sum wait for one another
+            float s[HT][KT][4], s2[HT][KT][4];            // keys g and g + 8 of 16, heads 2 quad and 2 quad + 1
 #pragma unroll
             for (int m = 0; m < HT; ++m)
 #pragma unroll
                 for (int j = 0; j < KT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[m][j][e] = 0.f;
+                    for (int e = 0; e < 4; ++e) s[m][j][e] = s2[m][j][e] = 0.f;
 #pragma unroll
             for (int j = 0; j < KT; ++j) {
                 if (!Cfg::CODES) {
@@ -444,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
                         uint32_t r[4];
                         load4(r, from + place<ROW_BYTES>(j * 16 + (lane & 15), d * 2 + (lane >> 4)));
 #pragma unroll
-                        for (int m = 0; m < HT; ++m) frag::mma_f32<Cfg::BF16>(s[m][j], r, q[m][d]);
+                        for (int m = 0; m < HT; ++m) frag::mma_f32<Cfg::BF16>(CHAINS == 2 && d % 2 ? s2[m][j] : s[m][j], r, q[m][d]);
                     }
                 } else {
 #pragma unroll
@@ -457,30 +480,43 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
                             widen4(r[2 * i], w[0], w[2]);
                             widen4(r[2 * i + 1], w[1], w[3]);
 #pragma unroll
-                            for (int m = 0; m < HT; ++m) frag::mma_f32<false>(s[m][j], w, q[m][d + i]);
+                            for (int m = 0; m < HT; ++m) frag::mma_f32<false>(CHAINS == 2 && i ? s2[m][j] : s[m][j], w, q[m][d + i]);
                         }
                     }
                 }
             }
 
             // ---- softmax
-            const bool ragged = token0 + KEYS > now.span.end;
+            if (CHAINS == 2) {
+#pragma unroll
+                for (int m = 0; m < HT; ++m)
+#pragma unroll
+                    for (int j = 0; j < KT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[m][j][e] += s2[m][j][e];
+            }
+            if (token0 + KEYS > now.span.end) {
+#pragma unroll
+                for (int j = 0; j < KT; ++j)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        if (token0 + j * 16 + half * 8 + g >= now.span.end) {
+#pragma unroll
+                            for (int m = 0; m < HT; ++m) s[m][j][half * 2] = s[m][j][half * 2 + 1] = -INFINITY;
+                        }
+            }
             float most[HT][2];
             bool passed = false;
 #pragma unroll
             for (int m = 0; m < HT; ++m)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    most[m][e] = LOWEST;
+                    most[m][e] = s[m][0][e];
 #pragma unroll
                     for (int j = 0; j < KT; ++j)
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            float& x = s[m][j][half * 2 + e];
-                            x *= factor[m][e];
-                            if (ragged && token0 + j * 16 + half * 8 + g >= now.span.end) x = -INFINITY;
-                            most[m][e] = fmaxf(most[m][e], x);
-                        }
+                        for (int half = 0; half < 2; ++half) most[m][e] = fmaxf(most[m][e], s[m][j][half * 2 + e]);
+                    most[m][e] *= factor[m][e];
                     passed |= most[m][e] > top[m][e] + SLACK;
                 }
             if (__any_sync(0xffffffffu, passed)) {
@@ -505,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, (Config<T, C, DIM, HT>::CTAS)) paged_
                 for (int j = 0; j < KT; ++j)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float u = exp2_(s[m][j][half * 2] - top[m][0]), v = exp2_(s[m][j][half * 2 + 1] - top[m][1]);
+                        const float u = exp2_(fmaf(s[m][j][half * 2], factor[m][0], -top[m][0])), v = exp2_(fmaf(s[m][j][half * 2 + 1], factor[m][1], -top[m][1]));
                         total[m][0] += u, total[m][1] += v;
                         // the weights' one rounding: the product with the values takes 16-bit operands (f16 or bf16)
                         p[m][j][half] = transposed(frag::pack_f32<Cfg::BF16>(u, v));
@@ -664,8 +700,8 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     std::call_once(once[device], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM); });
     Record* records = static_cast<Record*>(a.workspace);
     float* pieces = reinterpret_cast<float*>(records + grid);
-    if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), records, pieces))) return r;
-    if (longest_of(a) <= WHOLE_TILES * Cfg::TILE) return 0;  // no head can have been cut
+    if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), Cfg::THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), records, pieces))) return r;
+    if (grid < sms * Cfg::CTAS && longest_of(a) <= WHOLE_TILES * Cfg::TILE) return 0;  // no head can have been cut
     const int group = min(a.heads / a.cache.kv_heads, static_cast<int>(Cfg::ROWS));
     const dim3 join_grid(grid, (group + JOIN_ROWS - 1) / JOIN_ROWS);
     return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, HT>, join_grid, JOIN_WARPS * 32, 0, stream, a, records, pieces));

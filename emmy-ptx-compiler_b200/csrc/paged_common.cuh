@@ -72,9 +72,10 @@ inline int check_cache(const char* who, const emb_paged_cache_t& c, int q_dtype)
     return 0;
 }
 
-// Every kernel here is launched as a programmatic dependent of the work before it in the stream: its CTAs may be placed
-// while that work drains, which hides the launch, and before its first access to memory it waits until that work is
-// complete and visible (follow_on); at the same time it lets its own successor do the same.
+// Every kernel here is launched as a programmatic dependent of the work before it in the stream: it starts as that work's
+// CTAs end, and before its first access to memory it waits until the work is complete and visible (follow_on). None of them
+// lets its successor start earlier: CTAs that only wait then hold places that the running kernel's successors need (an
+// early launch_dependents cost attend 2 to 43 % of a pass back to back, and assign half of one).
 template <class... P, class... A> inline cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned block, unsigned smem, cudaStream_t stream, A... args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = grid, config.blockDim = dim3(block), config.dynamicSmemBytes = smem, config.stream = stream;
@@ -85,7 +86,7 @@ template <class... P, class... A> inline cudaError_t launch(void (*kernel)(P...)
     return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
 }
 __device__ __forceinline__ void follow_on() {
-    asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 struct E4m3 {

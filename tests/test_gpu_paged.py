@@ -397,7 +397,9 @@ def test_attend_bad_pages_and_lengths_show(paged):
     """A table entry outside the cache, and a length beyond the table row, are NaN in their request; a negative length is 0."""
     s = make_attend([200, 200, 200, 200], 4, 2, 64, BF16, BF16, 16)
     clean = paged.attend(**s)
-    s["table"][0, 3] = -5
+    for bad in (-1, -5, -2 ** 31):
+        s["table"][0, 3] = bad
+        assert paged.attend(**s)[0].isnan().all()
     s["table"][1, 12] = s["k_pages"].shape[0]
     s["lengths"][2] = 16 * s["table"].shape[1] + 1
     got = paged.attend(**s)
