@@ -5,6 +5,7 @@
 // were measured that way); here they are reads of the tensor's own fields. emmy_ptx/paged.py has the documented functions.
 
 #include <ATen/ops/empty.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -315,8 +316,11 @@ PyObject* attend(PyObject* const* o) {
     }
     a.out = out.given() ? out->data_ptr() : made.data_ptr();
     // a workspace of the call's own from torch's allocator: calls on other streams and captured graphs never share one
-    const at::Tensor workspace = empty({a.workspace_bytes}, at::kByte, device);
-    a.workspace = workspace.data_ptr();
+    c10::DataPtr workspace;
+    if (a.workspace_bytes) {
+        workspace = c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(a.workspace_bytes));
+        a.workspace = workspace.get();
+    }
     check(emb_paged_attend(&a, c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream()));
     if (!out.given()) return THPVariable_Wrap(std::move(made));
     Py_INCREF(o[9]);

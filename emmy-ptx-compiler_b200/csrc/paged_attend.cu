@@ -60,20 +60,11 @@ template <class T, class C, int DIM_, int HT_> struct Config {
     static_assert(CTAS * (SMEM + 1024 + 128) <= 228 * 1024, "shared memory of an SM");
 };
 
-// division by a number known to the host: floor(x / d) for x < 2^31
-struct Divisor {
-    uint32_t d, magic, shift;
-    explicit Divisor(uint32_t d_) : d(d_) {
-        shift = 0;
-        while ((1ull << shift) < d) ++shift;
-        magic = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-    }
-    __device__ __forceinline__ uint32_t over(uint32_t x) const { return (__umulhi(x, magic) + x) >> shift; }
-};
-
-// where a piece's rows lie: the record of a CTA whose last head goes on in the next CTAs, and two pieces a CTA
+// A head that was cut: the CTA that holds its first tiles and how many hold one (0: nothing to join). A CTA has two places
+// for pieces: the head that an earlier CTA began, and the head that goes on in later ones. A list has one record for each
+// CTA (of the head that goes on), or one for each head where there are fewer heads than CTAs.
 struct Record {
-    int32_t request, head, pieces, unused;  // head: of the cut work (key head, row group); pieces 0: nothing to join
+    int32_t request, head, cta, pieces;
 };
 
 struct Heads {  // how query heads fall on the rows of a CTA
@@ -175,7 +166,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 
 template <class T, class C, int DIM, int HT>
-__global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C, DIM, HT>::CTAS)) paged_attend_kernel(const emb_paged_attend_t a, const Divisor page_size, Record* __restrict__ records, float* __restrict__ pieces) {
+__global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C, DIM, HT>::CTAS)) paged_attend_kernel(const emb_paged_attend_t a, const Divisor page_size, Record* __restrict__ records, bool by_head, float* __restrict__ pieces) {
     using Cfg = Config<T, C, DIM, HT>;
     constexpr int WARPS = Cfg::WARPS, THREADS = Cfg::THREADS, KEYS = Cfg::KEYS, KT = KEYS / 16, DT = DIM / 16, ROW_BYTES = Cfg::ROW_BYTES, STAGES = Cfg::STAGES;
     constexpr int LOOKS = (KEYS + 31) / 32;  // keys that a lane looks up per step
@@ -216,7 +207,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     }
     const long long n = min(static_cast<long long>(gridDim.x), all);
     if (static_cast<long long>(blockIdx.x) >= n) {
-        if (tid == 0) records[blockIdx.x].pieces = 0;
+        if (tid == 0 && records && !by_head) records[blockIdx.x].pieces = 0;
         return;
     }
     const uint32_t whole = all <= static_cast<long long>(gridDim.x) ? WHOLE_TILES : 0;
@@ -241,7 +232,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     __syncthreads();
     const long long x0 = share[0], x1 = share[1];
     if (x0 >= x1) {
-        if (tid == 0) records[blockIdx.x].pieces = 0;
+        if (tid == 0 && records && !by_head) records[blockIdx.x].pieces = 0;
         return;
     }
     Cursor ahead;
@@ -441,7 +432,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     begin_head();
     int stage = 0;
     bool cut_in_front = now.t > 0;  // the head's tiles before these belong to an earlier CTA
-    Record record{0, 0, 0, 0};
+    Record record{0, 0, 0, 0};  // of the head that goes on
     for (long long step = 0; step < steps; ++step) {
         frag::cp_async_wait<STAGES - 2>();
         __syncwarp();
@@ -587,25 +578,26 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
             end_head(piece);
             if (!head_ends && !cut_in_front) {  // the head starts here and goes on: the CTAs up to the one that holds its last tile
                 const long long last = x1 - 1 + (now.tiles - 1 - now.t);
-                record = {now.b, now.head, static_cast<int>(((last + 1) * n + all - 1) / all - 1 - blockIdx.x + 1), 0};
+                record = {now.b, now.head, static_cast<int>(blockIdx.x), static_cast<int>(((last + 1) * n + all - 1) / all - 1 - blockIdx.x + 1)};
             }
+            if (by_head && tid == 0 && !cut_in_front) records[now.b * heads.cut + now.head] = head_ends ? Record{0, 0, 0, 0} : record;
             cut_in_front = false;
         }
         advance<Cfg>(now, a, heads.cut);
         if (head_ends && !share_ends) begin_head();
     }
-    if (tid == 0) records[blockIdx.x] = record;
+    if (tid == 0 && records && !by_head) records[blockIdx.x] = record;
 }
 
-// The pieces of the heads that were cut: CTA c adds up those of the head that starts in CTA c's share and goes on. A row's
-// maximum and sum are joined as in the kernel above. A row's pieces are dealt to JOIN_SPLIT warps, whose parts are added in
-// order: always the same order, so results do not depend on timing.
-constexpr int JOIN_WARPS = 8, JOIN_ROWS = 4, JOIN_SPLIT = JOIN_WARPS / JOIN_ROWS;
+// The pieces of the heads that were cut, a record and some rows of it for each CTA. A row's maximum and sum are joined as
+// in the kernel above. A row's pieces are dealt to `split` warps, whose parts are added in order: always the same order, so
+// results do not depend on timing. What it takes is the latency of three dependent loads, if a warp has few pieces.
+constexpr int JOIN_WARPS = 8;
 
 template <class T, class C, int DIM, int HT>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_paged_attend_t a, const Record* records, const float* pieces) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_paged_attend_t a, const Record* records, const float* pieces, int split) {
     using Cfg = Config<T, C, DIM, HT>;
-    constexpr int PER_LANE = DIM / 32;  // dims of a lane: two of DIM 64, else fours
+    constexpr int PER_LANE = DIM / 32;
     __shared__ float slab[JOIN_WARPS][Cfg::PITCH];
     follow_on();
     const Record record = records[blockIdx.x];
@@ -613,57 +605,60 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_p
     const Heads heads(a, Cfg::ROWS);
     const int kv = record.head / heads.groups, row0 = (record.head % heads.groups) * Cfg::ROWS;
     const int rows = min(Cfg::ROWS, heads.group - row0);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % JOIN_SPLIT;
-    for (int base = blockIdx.y * JOIN_ROWS; base < rows; base += gridDim.y * JOIN_ROWS) {
-        const int r = min(base + warp / JOIN_SPLIT, rows - 1);
-        const auto piece_of = [&](int i) { return pieces + (2ll * (blockIdx.x + i) + (i == 0)) * (Cfg::ROWS * Cfg::PITCH) + r * Cfg::PITCH; };
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % split, at_once = JOIN_WARPS / split;
+    for (int base = blockIdx.y * at_once; base < rows; base += gridDim.y * at_once) {
+        const int r = min(base + warp / split, rows - 1);
+        // piece i: the first in its CTA's second place, the others in their CTAs' first
+        const float* const from = pieces + 2ll * record.cta * (Cfg::ROWS * Cfg::PITCH) + r * Cfg::PITCH;
+        const auto piece = [&](int i) { return from + (2 * i + (i == 0)) * static_cast<long long>(Cfg::ROWS * Cfg::PITCH); };
         float best = LOWEST;
-        for (int k = lane; k < record.pieces; k += 32) best = fmaxf(best, piece_of(k)[DIM]);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+        for (int k = lane; k < record.pieces; k += 32) best = fmaxf(best, piece(k)[DIM]);
         float acc[PER_LANE] = {}, s = 0.f;
-#pragma unroll 8
-        for (int k = part; k < record.pieces; k += JOIN_SPLIT) {
-            const float* from = piece_of(k);
-            const float2 stat = *reinterpret_cast<const float2*>(from + DIM);
-            const float f = exp2_(stat.x - best);
+        constexpr int BATCH = 4;
+        bool seen = false;
+        for (int k0 = part; k0 < record.pieces; k0 += BATCH * split) {
+            float x[BATCH][PER_LANE], top[BATCH], sum[BATCH];
 #pragma unroll
-            for (int e = 0; e < PER_LANE; ++e) acc[e] += f * from[e * 32 + lane];
-            s += f * stat.y;
+            for (int u = 0; u < BATCH; ++u) {
+                const float* const p = piece(min(k0 + u * split, record.pieces - 1));
+                top[u] = p[DIM], sum[u] = p[DIM + 1];
+#pragma unroll
+                for (int e = 0; e < PER_LANE; ++e) x[u][e] = p[e * 32 + lane];
+            }
+            if (!seen) {  // (behind the first batch's loads)
+#pragma unroll
+                for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+                seen = true;
+            }
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                if (k0 + u * split >= record.pieces) break;
+                const float f = exp2_(top[u] - best);
+#pragma unroll
+                for (int e = 0; e < PER_LANE; ++e) acc[e] += f * x[u][e];
+                s += f * sum[u];
+            }
+        }
+        if (!seen) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
         }
         __syncthreads();  // the last rows' parts are read
 #pragma unroll
         for (int e = 0; e < PER_LANE; ++e) slab[warp][e * 32 + lane] = acc[e];
         if (lane == 0) slab[warp][DIM] = s;
         __syncthreads();
-        if (part == 0 && base + warp / JOIN_SPLIT < rows) {
+        if (part == 0 && base + warp / split < rows) {
             s = 0.f;
-#pragma unroll
-            for (int w = 0; w < JOIN_SPLIT; ++w) s += slab[warp + w][DIM];
+            for (int w = 0; w < split; ++w) s += slab[warp + w][DIM];
             for (int d = lane * 4; d < DIM; d += 128) {
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
                 float none = 0.f;
-#pragma unroll
-                for (int w = 0; w < JOIN_SPLIT; ++w) add_part(sum, none, *reinterpret_cast<const float4*>(&slab[warp + w][d]), 1.f, 0.f);
+                for (int w = 0; w < split; ++w) add_part(sum, none, *reinterpret_cast<const float4*>(&slab[warp + w][d]), 1.f, 0.f);
                 put_out<Cfg, T>(a, record.request, static_cast<long long>(kv) * heads.group + row0 + r, d, sum, best, s);
             }
         }
     }
-}
-
-constexpr int MAX_DEVICES = 64;
-
-// SMs of the current device; 0 and an error text where that cannot be had
-int sm_count() {
-    static int known[MAX_DEVICES];  // (threads that race here store the same number)
-    int device = -1;
-    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= MAX_DEVICES) return 0;
-    if (!known[device]) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
-        known[device] = n;
-    }
-    return known[device];
 }
 
 template <class Cfg> int64_t piece_bytes() { return 2ll * Cfg::ROWS * Cfg::PITCH * 4; }
@@ -686,25 +681,30 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     const int sms = sm_count();
     if (!sms) return refuse("paged_attend: the current device cannot be asked for its SMs");
     const int grid = grid_of<Cfg>(a, sms);
-    const int64_t bytes = grid * (static_cast<int64_t>(sizeof(Record)) + piece_bytes<Cfg>());
+    const bool cuts = grid == sms * Cfg::CTAS || longest_of(a) > WHOLE_TILES * Cfg::TILE;  // else no head is cut
+    const int64_t cut_heads = static_cast<int64_t>(a.requests) * Heads(a, Cfg::ROWS).cut;
+    const bool by_head = cuts && cut_heads <= grid;
+    const int64_t bytes = cuts ? grid * (static_cast<int64_t>(sizeof(Record)) + piece_bytes<Cfg>()) : 0;
     if (need) {
         *need = bytes;
         return 0;
     }
-    if (a.workspace_bytes < bytes || !a.workspace || !aligned16(a.workspace))
+    if (bytes && (a.workspace_bytes < bytes || !a.workspace || !aligned16(a.workspace)))
         return refuse("paged_attend: a workspace of %lld bytes (16-byte aligned) is needed, not %lld", static_cast<long long>(bytes), static_cast<long long>(a.workspace_bytes));
     auto kernel = paged_attend_kernel<T, C, DIM, HT>;
     static std::once_flag once[MAX_DEVICES];
     int device = 0;
     cudaGetDevice(&device);
     std::call_once(once[device], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM); });
-    Record* records = static_cast<Record*>(a.workspace);
+    Record* records = cuts ? static_cast<Record*>(a.workspace) : nullptr;
     float* pieces = reinterpret_cast<float*>(records + grid);
-    if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), Cfg::THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), records, pieces))) return r;
-    if (grid < sms * Cfg::CTAS && longest_of(a) <= WHOLE_TILES * Cfg::TILE) return 0;  // no head can have been cut
-    const int group = min(a.heads / a.cache.kv_heads, static_cast<int>(Cfg::ROWS));
-    const dim3 join_grid(grid, (group + JOIN_ROWS - 1) / JOIN_ROWS);
-    return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, HT>, join_grid, JOIN_WARPS * 32, 0, stream, a, records, pieces));
+    if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), Cfg::THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), records, by_head, pieces))) return r;
+    if (!cuts) return 0;
+    // about four CTAs an SM where records are few, each with as many warps for a row as its rows leave
+    const int list = by_head ? static_cast<int>(cut_heads) : grid, rows = std::min(a.heads / a.cache.kv_heads, static_cast<int>(Cfg::ROWS));
+    const int parts = std::max(1, std::min(rows, 4 * sms / list)), rows_each = (rows + parts - 1) / parts;
+    const int split = rows_each >= 8 ? 1 : rows_each > 2 ? 2 : rows_each > 1 ? 4 : 8;
+    return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, HT>, dim3(list, parts), JOIN_WARPS * 32, 0, stream, a, records, pieces, split));
 }
 
 template <class T, class C> int run_dim(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {

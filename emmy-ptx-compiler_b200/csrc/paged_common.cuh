@@ -72,6 +72,32 @@ inline int check_cache(const char* who, const emb_paged_cache_t& c, int q_dtype)
     return 0;
 }
 
+constexpr int MAX_DEVICES = 64;
+
+// SMs of the current device; 0 where that cannot be had
+inline int sm_count() {
+    static int known[MAX_DEVICES];  // (threads that race here store the same number)
+    int device = -1;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= MAX_DEVICES) return 0;
+    if (!known[device]) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+        known[device] = n;
+    }
+    return known[device];
+}
+
+// division by a number known to the host: floor(x / d) for x < 2^31
+struct Divisor {
+    uint32_t d, magic, shift;
+    explicit Divisor(uint32_t d_) : d(d_) {
+        shift = 0;
+        while ((1ull << shift) < d) ++shift;
+        magic = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t over(uint32_t x) const { return (__umulhi(x, magic) + x) >> shift; }
+};
+
 // Every kernel here is launched as a programmatic dependent of the work before it in the stream: it starts as that work's
 // CTAs end, and before its first access to memory it waits until the work is complete and visible (follow_on). None of them
 // lets its successor start earlier: CTAs that only wait then hold places that the running kernel's successors need (an
@@ -93,65 +119,40 @@ struct E4m3 {
     uint8_t code;
 };
 
-// eight consecutive elements of a row <-> f32; a load is one 16-byte (8-byte for codes) access
-template <class T> struct Vec8;
+// four consecutive elements of a row <-> f32
+template <class T> struct Vec4;
 
-template <> struct Vec8<__half> {
-    using raw = uint4;
-    static __device__ __forceinline__ void widen(const raw& r, float (&x)[8]) {
-        const __half2* h = reinterpret_cast<const __half2*>(&r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(h[i]);
-            x[2 * i] = f.x, x[2 * i + 1] = f.y;
-        }
-    }
-    static __device__ __forceinline__ raw narrow(const float (&x)[8]) {
-        raw r;
-        __half2* h = reinterpret_cast<__half2*>(&r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-        return r;
-    }
-};
-
-template <> struct Vec8<__nv_bfloat16> {
-    using raw = uint4;
-    static __device__ __forceinline__ void widen(const raw& r, float (&x)[8]) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(h[i]);
-            x[2 * i] = f.x, x[2 * i + 1] = f.y;
-        }
-    }
-    static __device__ __forceinline__ raw narrow(const float (&x)[8]) {
-        raw r;
-        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-        return r;
-    }
-};
-
-template <> struct Vec8<E4m3> {
+template <> struct Vec4<__half> {
     using raw = uint2;
-    static __device__ __forceinline__ void widen(const raw& r, float (&x)[8]) {
-        const __nv_fp8x2_storage_t* c = reinterpret_cast<const __nv_fp8x2_storage_t*>(&r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 h(__nv_cvt_fp8x2_to_halfraw2(c[i], __NV_E4M3));  // exact: e4m3 is a subset of f16
-            const float2 f = __half22float2(h);
-            x[2 * i] = f.x, x[2 * i + 1] = f.y;
-        }
+    static __device__ __forceinline__ void widen(const raw& r, float* x) {
+        const float2 lo = __half22float2(reinterpret_cast<const __half2&>(r.x)), hi = __half22float2(reinterpret_cast<const __half2&>(r.y));
+        x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
     }
+    static __device__ __forceinline__ raw narrow(const float* x) {
+        const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
+        return make_uint2(reinterpret_cast<const uint32_t&>(lo), reinterpret_cast<const uint32_t&>(hi));
+    }
+};
+
+template <> struct Vec4<__nv_bfloat16> {
+    using raw = uint2;
+    static __device__ __forceinline__ void widen(const raw& r, float* x) {
+        x[0] = __uint_as_float(r.x << 16), x[1] = __uint_as_float(r.x & 0xffff0000u);
+        x[2] = __uint_as_float(r.y << 16), x[3] = __uint_as_float(r.y & 0xffff0000u);
+    }
+    static __device__ __forceinline__ raw narrow(const float* x) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+        return make_uint2(reinterpret_cast<const uint32_t&>(lo), reinterpret_cast<const uint32_t&>(hi));
+    }
+};
+
+template <> struct Vec4<E4m3> {
+    using raw = uint32_t;
     // nearest even, saturating at +-448; NaN stays NaN
-    static __device__ __forceinline__ raw narrow(const float (&x)[8]) {
-        raw r;
-        __nv_fp8x2_storage_t* c = reinterpret_cast<__nv_fp8x2_storage_t*>(&r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-        return r;
+    static __device__ __forceinline__ raw narrow(const float* x) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
     }
 };
 

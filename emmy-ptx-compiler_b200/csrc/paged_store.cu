@@ -3,9 +3,17 @@
 //
 //   y = x / sqrt(mean(x^2) + eps) * weight;  pairs (a, b) of the first `rot` dims -> (a c - b s, b c + a s)
 //
-// Bound by HBM on prompts: every element is read once and written once, so a head row stays in registers from its load to
-// its store: LANES = dim / 8 lanes hold eight elements each (one 16-byte access), the mean is a butterfly over them, and
-// in the half-split rotation an element's partner is in the same register of the lane rot / 16 away.
+// Bound by HBM on prompts: every element is read once and written once. A head row stays in registers from its load to its
+// store: LANES = dim / 8 lanes hold two pieces of four elements each, chosen so that both elements of every pair to be
+// rotated are in one lane (pieces j and rot/2 + j of the rotated dims, or eight neighbours), and the mean of squares is a
+// butterfly over the lanes. With the norm's weight w, what a row's pair becomes is linear in it but for the norm:
+//   a' = r (a [w_a c] - b [w_b s]),  b' = r (b [w_b c] + a [w_a s]),  r = 1 / sqrt(mean + eps)
+// and the brackets are a token's and not a row's: a group of LANES lanes takes up to MOST_HEADS heads of one token, AHEAD
+// of them loaded at a time, and has the brackets, the slot and the addresses ready for all of them. A group has heads of one
+// kind only (q, k or v). (With the elements in order, the partners fetched by shuffles and heads of all kinds in a group the
+// arithmetic took longer than HBM: 130 us against 64 for 16384 tokens of 32 + 8 + 8 heads of 128, bf16.)
+
+#include <algorithm>
 
 #include "paged_common.cuh"
 
@@ -13,96 +21,149 @@ namespace {
 
 using namespace emb::paged;
 
-constexpr int THREADS = 128;
+constexpr int THREADS = 128, AHEAD = 4, MOST_HEADS = 8;
 
-template <class T, class C, int LANES> __global__ void __launch_bounds__(THREADS) paged_store_kernel(const emb_paged_store_t a) {
-    const int lane = threadIdx.x % LANES;
-    follow_on();
-    const int all_heads = a.heads + 2 * a.cache.kv_heads;
-    const long long rows = static_cast<long long>(a.tokens) * all_heads;
-    const long long row = static_cast<long long>(blockIdx.x) * (THREADS / LANES) + threadIdx.x / LANES;
-    const bool real = row < rows;
-    const int i = real ? static_cast<int>(row / all_heads) : 0;
-    const int h = real ? static_cast<int>(row % all_heads) : 0;
-    const bool is_q = h < a.heads, is_v = h >= a.heads + a.cache.kv_heads;
-    const int kv = is_q ? 0 : is_v ? h - a.heads - a.cache.kv_heads : h - a.heads;
-    const T* from = is_q   ? static_cast<const T*>(a.q) + i * a.q_stride[0] + h * a.q_stride[1]
-                    : is_v ? static_cast<const T*>(a.v) + i * a.v_stride[0] + kv * a.v_stride[1]
-                           : static_cast<const T*>(a.k) + i * a.k_stride[0] + kv * a.k_stride[1];
-    float x[8];
-    Vec8<T>::widen(*reinterpret_cast<const uint4*>(from + lane * 8), x);
+// how a launch's groups fall on a token: chunks of `heads` heads of q, of k and of v behind one another
+struct Chunks {
+    Divisor all;
+    int heads, q, k;
+};
 
-    const void* weight = is_q ? a.q_weight : a.k_weight;
-    float sum = 0.f;
+__device__ __forceinline__ uint2 load_piece(const char* at) {  // not through the read-only path: q may be q_out
+    uint2 r;
+    asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(at) : "memory");
+    return r;
+}
+
+enum Kind { Q, K, V };
+
+// the rows of one group, C: the type they are stored in
+template <class T, class C, int LANES, bool INTERLEAVED>
+__device__ __forceinline__ void rows_of(const emb_paged_store_t& a, Kind kind, int count, const char* from, int64_t from_step, char* to, int64_t to_step, int i, uint32_t mask) {
+    const int lane = threadIdx.x % LANES, half = a.rot / 2;
+    const bool turns = kind != V && (INTERLEAVED ? lane * 8 : lane * 4) < (INTERLEAVED ? a.rot : half);
+    // the dims of this lane's pieces
+    const int d0 = INTERLEAVED ? lane * 8 : lane * 4 < half ? lane * 4 : a.rot + (lane * 4 - half) * 2;
+    const int d1 = !INTERLEAVED && lane * 4 < half ? half + d0 : d0 + 4;
+    const char* const from0 = from + d0 * 2;
+    const char* const from1 = from + d1 * 2;
+    char* const to0 = to + d0 * static_cast<int>(sizeof(C));
+    char* const to1 = to + d1 * static_cast<int>(sizeof(C));
+
+    uint2 raw[AHEAD][2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
+    for (int u = 0; u < AHEAD; ++u)
+        if (u < count) raw[u][0] = load_piece(from0 + u * from_step), raw[u][1] = load_piece(from1 + u * from_step);
+
+    const T* const weight = static_cast<const T*>(kind == Q ? a.q_weight : kind == K ? a.k_weight : nullptr);
+    // x'[e] = r (x[e] own[e] + x[partner of e] other[e])
+    float own[8], other[8];
 #pragma unroll
-    for (int d = LANES / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (weight && !is_v) {
-        const float inv = rsqrtf(sum / (LANES * 8) + a.eps);
-        float w[8];
-        Vec8<T>::widen(reinterpret_cast<const uint4*>(weight)[lane], w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
+    for (int e = 0; e < 8; ++e) own[e] = 1.f, other[e] = 0.f;
+    if (weight) {
+        Vec4<T>::widen(*reinterpret_cast<const uint2*>(weight + d0), own);
+        Vec4<T>::widen(*reinterpret_cast<const uint2*>(weight + d1), own + 4);
     }
-
-    if (a.rot) {
-        const int d0 = lane * 8, half = a.rot / 2;
-        const bool turns = d0 < a.rot && !is_v;
+    if (turns) {
         const int position = a.positions[i];
         const bool known = position >= 0 && position < a.rope_rows;
-        const float* angles = a.rope + static_cast<long long>(known ? position : 0) * a.rot;
-        const float nan = __int_as_float(0x7fffffff);
-        if (a.interleaved) {
-            if (turns) {
+        const float* const angles = a.rope + static_cast<long long>(known ? position : 0) * a.rot + lane * 4;
+        const float4 c4 = *reinterpret_cast<const float4*>(angles), s4 = *reinterpret_cast<const float4*>(angles + half);
+        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const float c = known ? angles[d0 / 2 + p] : nan, s = known ? angles[half + d0 / 2 + p] : nan;
-                    const float u = x[2 * p], w = x[2 * p + 1];
-                    x[2 * p] = u * c - w * s, x[2 * p + 1] = w * c + u * s;
-                }
-            }
-        } else {
-            const bool low = d0 < half;
-            const int group = (threadIdx.x & 31) / LANES * LANES;
-            const int partner = group + (!turns ? lane : low ? lane + half / 8 : lane - half / 8);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float other = __shfl_sync(0xffffffffu, x[e], partner);
-                if (turns) {
-                    const int j = (low ? d0 : d0 - half) + e;
-                    const float c = known ? angles[j] : nan, s = known ? angles[half + j] : nan;
-                    x[e] = low ? x[e] * c - other * s : x[e] * c + other * s;
-                }
-            }
+        for (int p = 0; p < 4; ++p) {
+            const int x = INTERLEAVED ? 2 * p : p, y = INTERLEAVED ? 2 * p + 1 : p + 4;
+            const float cosine = known ? c[p] : __int_as_float(0x7fffffff), wx = own[x], wy = own[y];
+            own[x] = wx * cosine, other[x] = -wy * s[p];
+            own[y] = wy * cosine, other[y] = wx * s[p];
         }
     }
-    if (!real) return;
-    if (is_q) {
-        T* to = static_cast<T*>(a.q_out) + i * a.out_stride[0] + h * a.out_stride[1];
-        reinterpret_cast<uint4*>(to)[lane] = Vec8<T>::narrow(x);
+    const float unit = sizeof(C) == 1 ? 1.f / (kind == K ? a.cache.k_scale : a.cache.v_scale) : 1.f;
+
+    for (int h0 = 0; h0 < count; h0 += AHEAD) {
+        if (h0) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                if (h0 + u < count) raw[u][0] = load_piece(from0 + (h0 + u) * from_step), raw[u][1] = load_piece(from1 + (h0 + u) * from_step);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (h0 + u >= count) break;
+            char* const out0 = to0 + (h0 + u) * to_step;
+            char* const out1 = to1 + (h0 + u) * to_step;
+            if (sizeof(C) == 2 && kind == V) {
+                *reinterpret_cast<uint2*>(out0) = raw[u][0], *reinterpret_cast<uint2*>(out1) = raw[u][1];
+                continue;
+            }
+            float x[8], r = unit;
+            Vec4<T>::widen(raw[u][0], x);
+            Vec4<T>::widen(raw[u][1], x + 4);
+            if (weight) {
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+#pragma unroll
+                for (int d = LANES / 2; d; d >>= 1) sum += __shfl_xor_sync(mask, sum, d);
+                r *= rsqrtf(fmaf(sum, 1.f / (LANES * 8), a.eps));
+            }
+            float y[8];
+            if (turns) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int partner = INTERLEAVED ? e ^ 1 : e ^ 4;
+                    y[e] = r * fmaf(x[e], own[e], x[partner] * other[e]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = r * (x[e] * own[e]);
+            }
+            *reinterpret_cast<typename Vec4<C>::raw*>(out0) = Vec4<C>::narrow(y);
+            *reinterpret_cast<typename Vec4<C>::raw*>(out1) = Vec4<C>::narrow(y + 4);
+        }
+    }
+}
+
+template <class T, class C, int LANES, bool INTERLEAVED>
+__global__ void __launch_bounds__(THREADS, 6) paged_store_kernel(const emb_paged_store_t a, const Chunks chunks) {
+    const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);  // the group's lanes
+    follow_on();
+    const uint32_t work = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, i = chunks.all.over(work);
+    if (i >= static_cast<uint32_t>(a.tokens)) return;
+    const int chunk = work - i * chunks.all.d;
+    if (chunk < chunks.q) {
+        const int h = chunk * chunks.heads;
+        rows_of<T, T, LANES, INTERLEAVED>(a, Q, min(chunks.heads, a.heads - h), static_cast<const char*>(a.q) + (i * a.q_stride[0] + h * a.q_stride[1]) * 2, a.q_stride[1] * 2,
+                                          static_cast<char*>(a.q_out) + (i * a.out_stride[0] + h * a.out_stride[1]) * 2, a.out_stride[1] * 2, i, mask);
         return;
     }
     const int slot = a.slots[i];
     if (slot < 0 || slot >= a.cache.pages * a.cache.page_size) return;
-    const long long page = slot / a.cache.page_size, in_page = slot % a.cache.page_size;
-    const int64_t* stride = is_v ? a.cache.v_stride : a.cache.k_stride;
-    if (a.cache.dtype == EMB_U8) {
-        const float scale = is_v ? a.cache.v_scale : a.cache.k_scale;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __fdiv_rn(x[e], scale);
-    }
-    C* to = static_cast<C*>(is_v ? a.cache.v : a.cache.k) + page * stride[0] + in_page * stride[1] + kv * stride[2];
-    reinterpret_cast<typename Vec8<C>::raw*>(to)[lane] = Vec8<C>::narrow(x);
+    const int64_t page = slot / a.cache.page_size, in_page = slot % a.cache.page_size;
+    const bool is_k = chunk < chunks.q + chunks.k;
+    const int h = (chunk - chunks.q - (is_k ? 0 : chunks.k)) * chunks.heads;
+    const int64_t* const stride = is_k ? a.cache.k_stride : a.cache.v_stride;
+    const int64_t* const from_stride = is_k ? a.k_stride : a.v_stride;
+    constexpr int SIZE = sizeof(C);
+    rows_of<T, C, LANES, INTERLEAVED>(a, is_k ? K : V, min(chunks.heads, a.cache.kv_heads - h), static_cast<const char*>(is_k ? a.k : a.v) + (i * from_stride[0] + h * from_stride[1]) * 2, from_stride[1] * 2,
+                                      static_cast<char*>(is_k ? a.cache.k : a.cache.v) + (page * stride[0] + in_page * stride[1] + h * stride[2]) * SIZE, stride[2] * SIZE, i, mask);
+}
+
+template <class T, class C, int LANES> int run(const emb_paged_store_t& a, cudaStream_t stream) {
+    constexpr int GROUPS = THREADS / LANES;
+    const int sms = sm_count();
+    if (!sms) return refuse("paged_store: the current device cannot be asked for its SMs");
+    // a head per group while there are fewer rows than places for groups, then more
+    const int64_t rows = static_cast<int64_t>(a.tokens) * (a.heads + 2 * a.cache.kv_heads), places = static_cast<int64_t>(sms) * 6 * GROUPS;
+    const int heads = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows / places, MOST_HEADS)));
+    const int q = (a.heads + heads - 1) / heads, k = (a.cache.kv_heads + heads - 1) / heads, all = q + 2 * k;
+    const int64_t work = static_cast<int64_t>(a.tokens) * all;
+    if (work >= (1ll << 31) - GROUPS) return refuse("paged_store: %d rows of %d heads in one call", a.tokens, a.heads);
+    const auto kernel = a.interleaved ? paged_store_kernel<T, C, LANES, true> : paged_store_kernel<T, C, LANES, false>;
+    return launched("launch of paged_store", launch(kernel, dim3(static_cast<unsigned>((work + GROUPS - 1) / GROUPS)), THREADS, 0, stream, a, Chunks{Divisor(all), heads, q, k}));
 }
 
 template <class T, class C> int run_dim(const emb_paged_store_t& a, cudaStream_t stream) {
-    const long long rows = static_cast<long long>(a.tokens) * (a.heads + 2 * a.cache.kv_heads);
-    const int per_cta = THREADS / (a.cache.dim / 8);
-    const long long grid = (rows + per_cta - 1) / per_cta;
-    if (grid > 0x7fffffffll) return refuse("paged_store: %lld head rows in one call", rows);
-    const auto kernel = a.cache.dim == 64 ? paged_store_kernel<T, C, 8> : a.cache.dim == 128 ? paged_store_kernel<T, C, 16> : paged_store_kernel<T, C, 32>;
-    return launched("launch of paged_store", launch(kernel, static_cast<unsigned>(grid), THREADS, 0, stream, a));
+    return a.cache.dim == 64 ? run<T, C, 8>(a, stream) : a.cache.dim == 128 ? run<T, C, 16>(a, stream) : run<T, C, 32>(a, stream);
 }
 
 }  // namespace

@@ -260,8 +260,8 @@ int emb_paged_assign(const emb_paged_assign_t* args, void* stream);
  *   each position, rot/2 cosines and then rot/2 sines; pair j is (y[j], y[j+rot/2]),
  *   or (y[2j], y[2j+1]) where `interleaved`:  (a c - b s, b c + a s)
  * all in f32, rounded once: q_out[i, h] in q's type, keys and values (the values as
- * they are) into slot slots[i] of the cache in the cache's type (e4m3: divided by
- * the scale, nearest even, saturating). A slot outside the cache (negative among
+ * they are) into slot slots[i] of the cache in the cache's type (e4m3: times
+ * 1 / scale, nearest even, saturating). A slot outside the cache (negative among
  * them) stores nothing; its q_out is written. A position outside the table gives
  * NaN in the rotated dims. Two rows with the same slot: either's values. q_out may
  * be q. A cache of 16-bit type has q's type. */
