@@ -1,11 +1,14 @@
 // emb_paged_assign: page tables and slot maps of a serving step, from the requests' lengths, on the GPU.
 //
 // Two prefix sums over the requests (new rows, new pages) decide everything; no request's pages depend on a value that
-// another thread writes, so one launch does it: every CTA sums over all requests (lengths are a few KB and stay in L2)
-// and keeps the requests whose rows meet its own ROWS rows of the step; then a thread per row finds its request among
-// them by bisection. A page that is new to a request is entered into the table by the row that is its first token: the
-// page of a row behind it comes from the free list, not from the table, so rows never wait for one another.
-// Bound by latency (one launch, two dependent loads and a scan): the traffic is 8 bytes a row.
+// another thread writes, so one launch does it: every CTA sums over all requests (lengths are a few KB and stay in L2) and
+// takes ROWS rows of the step. A request that has rows there leaves what they need to know at the place of its first one; a
+// running maximum over the places then gives each row its request. A page that is new to a request is entered into the
+// table by the row that is its first token: the page of a row behind it comes from the free list, not from the table, so
+// rows never wait for one another. Sums saturate at 2^31 - 1, beyond anything that can be granted.
+// Bound by latency (a launch, loads of lengths, a scan, loads of pages): the traffic is 8 bytes a row. (One request a
+// thread, a scan for each sum and a bisection for each row took 12.2 us with a cold L2 for 1000 requests with up to 512
+// new tokens, where this takes 6.2; a kernel that does nothing takes 2.2 so measured.)
 
 #include "paged_common.cuh"
 
@@ -13,120 +16,141 @@ namespace {
 
 using namespace emb::paged;
 
-constexpr int THREADS = 256;
-constexpr int ROWS = 1024;  // rows of the step per CTA
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int ITEMS = 4;            // requests of a thread per pass
+constexpr int ROWS = 2 * THREADS;   // rows of the step per CTA
+constexpr uint32_t MOST = 0x7fffffffu;
 
-struct Meets {  // a request whose rows meet this CTA's
-    int32_t start, request, cached, have;
-    long long first;  // of its new pages in the free list; -1: refused
+struct Request {  // of a row
+    int32_t start, id, cached, have;
+    int32_t first, granted;  // its first new page's place in the free list
 };
 
-struct Sums {
-    long long x;
-    int32_t y;
-};
+__device__ __forceinline__ uint32_t sum_of(uint32_t a, uint32_t b) { return min(a + b, MOST); }
 
-__device__ __forceinline__ Sums operator+(const Sums& a, const Sums& b) { return {a.x + b.x, a.y + b.y}; }
-
-// inclusive sums over the CTA's threads in thread order, and over all of them
-__device__ __forceinline__ Sums block_scan(Sums v, Sums (&slab)[THREADS / 32], Sums& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, v.x, d);
-        const int32_t y = __shfl_up_sync(0xffffffffu, v.y, d);
-        if (lane >= d) v.x += x, v.y += y;
-    }
-    __syncthreads();  // the slab's last readers are done
-    if (lane == 31) slab[warp] = v;
-    __syncthreads();
-    Sums before{0, 0};
-    total = {0, 0};
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) before = before + slab[w];
-        total = total + slab[w];
-    }
-    return before + v;
-}
-
-__device__ __forceinline__ int32_t clamp_i32(long long x) { return x > 0x7fffffffll ? 0x7fffffff : static_cast<int32_t>(x); }
-
-__global__ void __launch_bounds__(THREADS) paged_assign_kernel(const emb_paged_assign_t a) {
-    __shared__ Meets meets[ROWS];  // in the requests' order; each of them has a row of this CTA's, so ROWS are enough
-    __shared__ Sums slab[THREADS / 32];
-    __shared__ long long taken_all;
-    __shared__ int refused_all;
-    const int tid = threadIdx.x;
+__global__ void __launch_bounds__(THREADS) paged_assign_kernel(const emb_paged_assign_t a, const Divisor page_size) {
+    __shared__ Request at[ROWS];
+    __shared__ int place[ROWS];  // of the request that starts at a row (or goes on at row 0): the row + 1; else 0
+    __shared__ uint32_t row_slab[WARPS], page_slab[WARPS];
+    __shared__ int top_slab[WARPS];
+    __shared__ unsigned taken_all, refused_all;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < ROWS; i += THREADS) place[i] = 0;
+    if (tid == 0) taken_all = refused_all = 0;
     follow_on();
-    const long long row0 = static_cast<long long>(blockIdx.x) * ROWS;
-    const long long row1 = min(row0 + ROWS, static_cast<long long>(a.tokens));
-    const long long head = min(max(*a.free_head, 0), a.free_count), room = a.free_count - head;
-    if (tid == 0) taken_all = 0, refused_all = 0;
+    const uint32_t row0 = blockIdx.x * ROWS, tokens = a.tokens, row1 = min(row0 + ROWS, tokens);
+    const uint32_t head = min(max(*a.free_head, 0), a.free_count), room = a.free_count - head;
+    const uint32_t capacity = static_cast<uint32_t>(a.table_width) * page_size.d;
+    const auto pages_for = [&](uint32_t n) { return n ? page_size.over(n - 1) + 1 : 0u; };
 
-    long long rows_done = 0, pages_done = 0, taken = 0;
-    int met = 0, refused = 0;
-    for (int base = 0; base < a.requests; base += THREADS) {
-        const int b = base + tid;
-        const bool real = b < a.requests;
-        const long long c = real ? max(a.cached[b], 0) : 0, f = real ? max(a.fresh[b], 0) : 0;
-        const long long have = (c + a.page_size - 1) / a.page_size, want = (c + f + a.page_size - 1) / a.page_size;
-        Sums total;
-        const long long end = rows_done + block_scan({f, 0}, slab, total).x, start = end - f;
-        rows_done += total.x;
-        const bool fits = f == 0 || (c + f <= static_cast<long long>(a.table_width) * a.page_size && end <= a.tokens);
-        const long long need = fits ? want - have : 0;
-        const bool meet = f > 0 && start < row1 && end > row0;
-        const Sums upto = Sums{pages_done, met} + block_scan({need, meet}, slab, total);
-        pages_done += total.x, met += total.y;
-        // the needs' running sum only grows, so the requests that get pages are those before the first one that does not
-        const bool granted = fits && (need == 0 || upto.x <= room);
-        refused += !granted;
-        if (granted && need) taken = upto.x;
-        if (meet) meets[upto.y - 1] = {static_cast<int32_t>(start), b, static_cast<int32_t>(c), static_cast<int32_t>(have), granted ? head + upto.x - need : -1};
-        if (real && blockIdx.x == 0) {
-            a.starts[b] = clamp_i32(start);
-            a.lengths[b] = clamp_i32(granted ? c + f : c);
+    uint32_t rows_done = 0, pages_done = 0, taken = 0, refused = 0;
+    for (int base = 0; base < a.requests; base += THREADS * ITEMS) {
+        uint32_t cached[ITEMS], fresh[ITEMS], have[ITEMS], need[ITEMS], rows = 0, pages = 0;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int b = base + tid * ITEMS + k;
+            cached[k] = b < a.requests ? max(a.cached[b], 0) : 0;
+            fresh[k] = b < a.requests ? max(a.fresh[b], 0) : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            have[k] = pages_for(cached[k]);
+            // (a request that does not fit its table row asks for nothing; one that does not fit the step's rows stands behind all
+            // that do, so what it asks for changes nothing)
+            need[k] = fresh[k] && cached[k] + fresh[k] <= capacity ? pages_for(cached[k] + fresh[k]) - have[k] : 0u;
+            rows = sum_of(rows, fresh[k]), pages = sum_of(pages, need[k]);
+        }
+        uint32_t rows_upto = rows, pages_upto = pages;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t r = __shfl_up_sync(0xffffffffu, rows_upto, d), p = __shfl_up_sync(0xffffffffu, pages_upto, d);
+            if (lane >= d) rows_upto = sum_of(rows_upto, r), pages_upto = sum_of(pages_upto, p);
+        }
+        // (what stands before this thread's requests; a saturated sum stays saturated: it is not taken back by a subtraction)
+        uint32_t row_before = __shfl_up_sync(0xffffffffu, rows_upto, 1), page_before = __shfl_up_sync(0xffffffffu, pages_upto, 1);
+        if (lane == 0) row_before = page_before = 0;
+        __syncthreads();  // the slabs' last readers are done, and `place` is cleared
+        if (lane == 31) row_slab[warp] = rows_upto, page_slab[warp] = pages_upto;
+        __syncthreads();
+        uint32_t start = rows_done, upto = pages_done;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) start = sum_of(start, row_slab[w]), upto = sum_of(upto, page_slab[w]);
+            rows_done = sum_of(rows_done, row_slab[w]), pages_done = sum_of(pages_done, page_slab[w]);
+        }
+        start = sum_of(start, row_before), upto = sum_of(upto, page_before);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int b = base + tid * ITEMS + k;
+            const uint32_t end = sum_of(start, fresh[k]), first = upto;
+            upto = sum_of(upto, need[k]);
+            // the needs' running sum only grows, so the requests that get pages are those before the first one that does not
+            const bool granted = !fresh[k] || (cached[k] + fresh[k] <= capacity && end <= tokens && (!need[k] || upto <= room));
+            refused += !granted;
+            if (granted && need[k]) taken = upto;
+            if (fresh[k] && start < row1 && end > row0) {
+                const uint32_t row = max(start, row0) - row0;
+                place[row] = row + 1;
+                at[row] = {static_cast<int32_t>(start), b, static_cast<int32_t>(cached[k]), static_cast<int32_t>(have[k]), static_cast<int32_t>(head + first), granted};
+            }
+            if (blockIdx.x == 0 && b < a.requests) {
+                a.starts[b] = start;
+                a.lengths[b] = granted ? cached[k] + fresh[k] : cached[k];
+            }
+            start = end;
         }
     }
-    __syncthreads();  // `meets` is whole
+    __syncthreads();  // `place` and `at` are whole
+
+    // the last place at or before each row; a thread has two rows side by side
+    const int p0 = place[tid * 2], p1 = max(p0, place[tid * 2 + 1]);
+    int upto = p1;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto = max(upto, x);
+    }
+    int before = __shfl_up_sync(0xffffffffu, upto, 1);
+    if (lane == 0) before = 0;
+    if (lane == 31) top_slab[warp] = upto;
     if (blockIdx.x == 0) {
         if (refused) atomicAdd(&refused_all, refused);
         if (taken) atomicMax(&taken_all, taken);
-        __syncthreads();
-        if (tid == 0) {
-            a.starts[a.requests] = clamp_i32(rows_done);
-            *a.free_head_out = static_cast<int32_t>(head + taken_all);
-            a.report[0] = static_cast<int32_t>(taken_all);
-            a.report[1] = refused_all;
-            a.report[2] = clamp_i32(max(rows_done - a.tokens, 0ll));
-            a.report[3] = clamp_i32(rows_done);
-        }
     }
-    for (long long i = row0 + tid; i < row1; i += THREADS) {
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+        if (w < warp) before = max(before, top_slab[w]);
+    if (blockIdx.x == 0 && tid == 0) {
+        a.starts[a.requests] = rows_done;
+        *a.free_head_out = head + taken_all;
+        a.report[0] = taken_all;
+        a.report[1] = refused_all;
+        a.report[2] = rows_done > tokens ? rows_done - tokens : 0;
+        a.report[3] = rows_done;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const uint32_t i = row0 + tid * 2 + u;
+        if (i >= row1) break;
+        const int from = max(before, u ? p1 : p0);
         int32_t slot = -1, position = 0;
-        if (i < rows_done) {
-            int lo = 0, hi = met;  // the last request that starts at or before row i
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (meets[mid].start <= i) lo = mid;
-                else hi = mid;
-            }
-            const Meets m = meets[lo];
-            const long long pos = m.cached + (i - m.start);
-            position = clamp_i32(pos);
-            if (m.first >= 0) {
-                const int32_t index = static_cast<int32_t>(pos / a.page_size), in_page = static_cast<int32_t>(pos % a.page_size);
-                int32_t* entry = a.table + m.request * a.table_stride + index;
+        if (i < rows_done && from) {
+            const Request r = at[from - 1];
+            const uint32_t pos = sum_of(r.cached, i - r.start);
+            position = pos;
+            if (r.granted) {
+                const uint32_t index = page_size.over(pos), in_page = pos - index * page_size.d;
+                int32_t* const entry = a.table + r.id * a.table_stride + index;
                 int32_t page;
-                if (index < m.have) {
+                if (index < static_cast<uint32_t>(r.have)) {
                     page = *entry;
                 } else {
-                    page = a.free_pages[m.first + index - m.have];
+                    page = a.free_pages[r.first + (index - r.have)];
                     if (in_page == 0) *entry = page;
                 }
-                const long long s = static_cast<long long>(page) * a.page_size + in_page;
-                if (page >= 0 && s <= 0x7fffffffll) slot = static_cast<int32_t>(s);
+                const long long s = static_cast<long long>(page) * page_size.d + in_page;
+                if (page >= 0 && s <= MOST) slot = static_cast<int32_t>(s);
             }
         }
         a.slots[i] = slot;
@@ -140,6 +164,7 @@ extern "C" int emb_paged_assign(const emb_paged_assign_t* args, void* stream) {
     if (!args) return refuse("paged_assign: null arguments");
     const emb_paged_assign_t& a = *args;
     if (static_cast<int64_t>(a.table_width) * a.page_size >= (1ll << 31)) return refuse("paged_assign: a table row of 2^31 tokens or more");
+    if (a.tokens > (1ll << 31) - 1024) return refuse("paged_assign: 2^31 rows or more");
     if (a.requests < 0 || a.table_width < 1 || a.free_count < 0 || a.page_size < 1 || a.tokens < 0 || a.table_stride < 0)
         return refuse("paged_assign: a count is negative, or the table width or page size below 1");
     if ((a.requests && (!a.cached || !a.fresh || !a.table || !a.lengths)) || (a.free_count && !a.free_pages) ||
@@ -149,5 +174,5 @@ extern "C" int emb_paged_assign(const emb_paged_assign_t* args, void* stream) {
     if (a.lengths && (a.lengths == a.cached || a.lengths == a.fresh)) return refuse("paged_assign: lengths may not be cached or fresh");
     if (a.free_head_out == a.free_head) return refuse("paged_assign: free_head_out may not be free_head");
     const unsigned grid = a.tokens > ROWS ? (static_cast<unsigned>(a.tokens) + ROWS - 1) / ROWS : 1u;
-    return launched("launch of paged_assign", launch(paged_assign_kernel, grid, THREADS, 0, static_cast<cudaStream_t>(stream), a));
+    return launched("launch of paged_assign", launch(paged_assign_kernel, dim3(grid), THREADS, 0, static_cast<cudaStream_t>(stream), a, Divisor(a.page_size)));
 }

@@ -8,8 +8,8 @@
 // rotated are in one lane (pieces j and rot/2 + j of the rotated dims, or eight neighbours), and the mean of squares is a
 // butterfly over the lanes. With the norm's weight w, what a row's pair becomes is linear in it but for the norm:
 //   a' = r (a [w_a c] - b [w_b s]),  b' = r (b [w_b c] + a [w_a s]),  r = 1 / sqrt(mean + eps)
-// and the brackets are a token's and not a row's: a group of LANES lanes takes up to MOST_HEADS heads of one token, AHEAD
-// of them loaded at a time, and has the brackets, the slot and the addresses ready for all of them. A group has heads of one
+// and the brackets are a token's and not a row's: a group of LANES lanes takes up to MOST_HEADS heads of one token, the
+// next AHEAD of them loaded while AHEAD are at work, and has the brackets, the slot and the addresses ready for all of them. A group has heads of one
 // kind only (q, k or v). (With the elements in order, the partners fetched by shuffles and heads of all kinds in a group the
 // arithmetic took longer than HBM: 130 us against 64 for 16384 tokens of 32 + 8 + 8 heads of 128, bf16.)
 
@@ -21,7 +21,7 @@ namespace {
 
 using namespace emb::paged;
 
-constexpr int THREADS = 128, AHEAD = 4, MOST_HEADS = 8;
+constexpr int THREADS = 128, AHEAD = 2, MOST_HEADS = 8;
 
 // how a launch's groups fall on a token: chunks of `heads` heads of q, of k and of v behind one another
 struct Chunks {
@@ -50,10 +50,13 @@ __device__ __forceinline__ void rows_of(const emb_paged_store_t& a, Kind kind, i
     char* const to0 = to + d0 * static_cast<int>(sizeof(C));
     char* const to1 = to + d1 * static_cast<int>(sizeof(C));
 
-    uint2 raw[AHEAD][2];
+    uint2 next[AHEAD][2];
+    const auto load = [&](int h0) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-        if (u < count) raw[u][0] = load_piece(from0 + u * from_step), raw[u][1] = load_piece(from1 + u * from_step);
+        for (int u = 0; u < AHEAD; ++u)
+            if (h0 + u < count) next[u][0] = load_piece(from0 + (h0 + u) * from_step), next[u][1] = load_piece(from1 + (h0 + u) * from_step);
+    };
+    load(0);
 
     const T* const weight = static_cast<const T*>(kind == Q ? a.q_weight : kind == K ? a.k_weight : nullptr);
     // x'[e] = r (x[e] own[e] + x[partner of e] other[e])
@@ -81,11 +84,10 @@ __device__ __forceinline__ void rows_of(const emb_paged_store_t& a, Kind kind, i
     const float unit = sizeof(C) == 1 ? 1.f / (kind == K ? a.cache.k_scale : a.cache.v_scale) : 1.f;
 
     for (int h0 = 0; h0 < count; h0 += AHEAD) {
-        if (h0) {
+        uint2 raw[AHEAD][2];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
-                if (h0 + u < count) raw[u][0] = load_piece(from0 + (h0 + u) * from_step), raw[u][1] = load_piece(from1 + (h0 + u) * from_step);
-        }
+        for (int u = 0; u < AHEAD; ++u) raw[u][0] = next[u][0], raw[u][1] = next[u][1];
+        load(h0 + AHEAD);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (h0 + u >= count) break;
@@ -124,7 +126,7 @@ __device__ __forceinline__ void rows_of(const emb_paged_store_t& a, Kind kind, i
 }
 
 template <class T, class C, int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(THREADS, 6) paged_store_kernel(const emb_paged_store_t a, const Chunks chunks) {
+__global__ void __launch_bounds__(THREADS, 8) paged_store_kernel(const emb_paged_store_t a, const Chunks chunks) {
     const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);  // the group's lanes
     follow_on();
     const uint32_t work = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, i = chunks.all.over(work);
@@ -153,7 +155,7 @@ template <class T, class C, int LANES> int run(const emb_paged_store_t& a, cudaS
     const int sms = sm_count();
     if (!sms) return refuse("paged_store: the current device cannot be asked for its SMs");
     // a head per group while there are fewer rows than places for groups, then more
-    const int64_t rows = static_cast<int64_t>(a.tokens) * (a.heads + 2 * a.cache.kv_heads), places = static_cast<int64_t>(sms) * 6 * GROUPS;
+    const int64_t rows = static_cast<int64_t>(a.tokens) * (a.heads + 2 * a.cache.kv_heads), places = static_cast<int64_t>(sms) * 8 * GROUPS;
     const int heads = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows / places, MOST_HEADS)));
     const int q = (a.heads + heads - 1) / heads, k = (a.cache.kv_heads + heads - 1) / heads, all = q + 2 * k;
     const int64_t work = static_cast<int64_t>(a.tokens) * all;
