@@ -87,7 +87,8 @@ __device__ __forceinline__ Span span_of(const emb_paged_attend_t& a, int b) {
     return {a.window && n > a.window ? n - a.window : 0u, n};
 }
 
-template <int TILE> __device__ __forceinline__ uint32_t tiles_of(const Span& s) { return max(1u, (s.end - s.begin + TILE - 1) / TILE); }
+// tiles begin at a multiple of 16 keys, at or before the first one
+template <int TILE> __device__ __forceinline__ uint32_t tiles_of(const Span& s) { return max(1u, (s.end - (s.begin & ~15u) + TILE - 1) / TILE); }
 
 struct Cursor {  // a tile of the CTA's share
     int b, head;
@@ -169,7 +170,7 @@ template <class T, class C, int DIM, int HT>
 __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C, DIM, HT>::CTAS)) paged_attend_kernel(const emb_paged_attend_t a, const Divisor page_size, Record* __restrict__ records, bool by_head, float* __restrict__ pieces) {
     using Cfg = Config<T, C, DIM, HT>;
     constexpr int WARPS = Cfg::WARPS, THREADS = Cfg::THREADS, KEYS = Cfg::KEYS, KT = KEYS / 16, DT = DIM / 16, ROW_BYTES = Cfg::ROW_BYTES, STAGES = Cfg::STAGES;
-    constexpr int LOOKS = (KEYS + 31) / 32;  // keys that a lane looks up per step
+    constexpr int LOOKS = (KEYS + 31) / 32;  // keys that a lane looks up per step, at most
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long scan_slab[WARPS], share[2];
     __shared__ long long first_before;  // tiles before the request that holds the share's first tile
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
         if (tid == 0 && records && !by_head) records[blockIdx.x].pieces = 0;
         return;
     }
-    const uint32_t whole = all <= static_cast<long long>(gridDim.x) ? WHOLE_TILES : 0;
+    const uint32_t whole = !pieces ? 0xffffffffu : all <= static_cast<long long>(gridDim.x) ? WHOLE_TILES : 0;  // no place for pieces: no cuts
     if (tid < 2) share[tid] = all * (blockIdx.x + tid) / n;
     __syncthreads();
     const long long want0 = share[0], want1 = share[1];
@@ -248,29 +249,41 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     const uint32_t k_stride[3] = {static_cast<uint32_t>(a.cache.k_stride[0]), static_cast<uint32_t>(a.cache.k_stride[1]), static_cast<uint32_t>(a.cache.k_stride[2])};
     const uint32_t v_stride[3] = {static_cast<uint32_t>(a.cache.v_stride[0]), static_cast<uint32_t>(a.cache.v_stride[1]), static_cast<uint32_t>(a.cache.v_stride[2])};
     const bool same = k_stride[0] == v_stride[0] && k_stride[1] == v_stride[1] && k_stride[2] == v_stride[2];
-    const auto token_of = [&](int look) { return ahead.span.begin + ahead.t * Cfg::TILE + warp * KEYS + look * 32 + (lane & (KEYS < 32 ? KEYS - 1 : 31)); };
-    // of this lane's keys, found a step before they are needed: the page id (-1: behind the length, -2: none) and the token in it
+    // where pages are multiples of 16 tokens, sixteen keys lie in one page behind one another: a lane looks up sixteen at a
+    // time, else one
+    const bool sixteens = page_size.d % 16 == 0;
+    const auto token_of = [&](int look) {
+        return (ahead.span.begin & ~15u) + ahead.t * Cfg::TILE + warp * KEYS + (sixteens ? lane % (KEYS / 16) * 16 : look * 32 + lane % min(KEYS, 32));
+    };
+    // found a step before they are needed: the page id (-1: behind the length, -2: none) and the token in it
     int page[LOOKS];
     uint32_t in_page[LOOKS];
     const auto find_pages = [&]() {
 #pragma unroll
         for (int l = 0; l < LOOKS; ++l) {
+            if (l && sixteens) break;
             const uint32_t token = token_of(l), index = page_size.over(token);
             in_page[l] = token - index * page_size.d;
             page[l] = -1;
-            if (token < ahead.span.end) {
+            if (token < ahead.span.end && (sixteens || token >= ahead.span.begin)) {
                 const uint32_t id = index < static_cast<uint32_t>(a.table_width) ? __ldg(a.table + ahead.b * a.table_stride + index) : -2;
                 page[l] = min(id, 0xfffffffeu);  // (an entry of -1 is a page that is not there, too)
             }
         }
     };
+    constexpr int CHUNKS = ROW_BYTES / 16, PER_PASS = 32 / CHUNKS;  // 16-byte pieces of a row; rows that the warp copies at once
+    const int chunk = lane % CHUNKS;
+    const unsigned long long k_step = k_stride[1] * sizeof(C), v_step = v_stride[1] * sizeof(C);  // bytes from a token to the next
+    const char* const k_from = static_cast<const char*>(a.cache.k) + chunk * 16;
+    const char* const v_from = static_cast<const char*>(a.cache.v) + chunk * 16;
     const auto issue = [&](int stage) {
         const uint32_t kv = ahead.head / heads.groups;
-        // byte offsets of the keys' rows (strides are below 2^32 elements), or the page id where there is no row
+        // byte offsets of the rows (strides are below 2^32 elements), or the page id where there is no row
         long long k_at[LOOKS], v_at[LOOKS];
         bool known = true;
 #pragma unroll
         for (int l = 0; l < LOOKS; ++l) {
+            if (l && sixteens) break;
             const bool one = static_cast<uint32_t>(page[l]) < static_cast<uint32_t>(a.cache.pages);
             const unsigned long long id = static_cast<uint32_t>(page[l]);
             k_at[l] = one ? (id * k_stride[0] + static_cast<unsigned long long>(in_page[l]) * k_stride[1] + static_cast<unsigned long long>(kv) * k_stride[2]) * sizeof(C) : page[l] == -1 ? -1 : -2;
@@ -278,22 +291,41 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
             if (!same && one) v_at[l] = (id * v_stride[0] + static_cast<unsigned long long>(in_page[l]) * v_stride[1] + static_cast<unsigned long long>(kv) * v_stride[2]) * sizeof(C);
             known = known && one;
         }
-        constexpr int CHUNKS = ROW_BYTES / 16, PER_PASS = 32 / CHUNKS;
         const uint32_t to = ring + stage * Cfg::STEP_BYTES;
-        const int chunk = lane % CHUNKS;
-        const char* const k_from = static_cast<const char*>(a.cache.k) + chunk * 16;
-        const char* const v_from = static_cast<const char*>(a.cache.v) + chunk * 16;
-        const bool all_known = __all_sync(0xffffffffu, known);
+        const uint32_t token0 = (ahead.span.begin & ~15u) + ahead.t * Cfg::TILE + warp * KEYS;
+        if (sixteens && __all_sync(0xffffffffu, known) && token0 >= ahead.span.begin && token0 + KEYS <= ahead.span.end) {
 #pragma unroll
+            for (int s = 0; s < KEYS / 16; ++s) {
+                const long long k_first = __shfl_sync(0xffffffffu, k_at[0], s), v_first = same ? k_first : __shfl_sync(0xffffffffu, v_at[0], s);
+                const char* k_row = k_from + k_first + (lane / CHUNKS) * k_step;
+                const char* v_row = v_from + v_first + (lane / CHUNKS) * v_step;
+#pragma unroll
+                for (int p = 0; p < 16 / PER_PASS; ++p) {
+                    const uint32_t k_to = to + place<ROW_BYTES>(s * 16 + p * PER_PASS + lane / CHUNKS, chunk);
+                    copy16<ROW_BYTES>(k_to, k_row);
+                    copy16<ROW_BYTES>(k_to + KEYS * ROW_BYTES, v_row);
+                    k_row += k_step * PER_PASS, v_row += v_step * PER_PASS;
+                }
+            }
+            return;
+        }
+        // row by row: the ends of a span, pages that are not there, pages of other sizes
+#pragma unroll 2
         for (int p = 0; p < KEYS / PER_PASS; ++p) {
-            const int row = p * PER_PASS + lane / CHUNKS;
-            const long long k_row = __shfl_sync(0xffffffffu, k_at[p * PER_PASS / 32], row & 31);
-            const long long v_row = same ? k_row : __shfl_sync(0xffffffffu, v_at[p * PER_PASS / 32], row & 31);
+            const int row = p * PER_PASS + lane / CHUNKS, source = sixteens ? row >> 4 : row & 31;
+            const bool second = LOOKS > 1 && !sixteens && row >= 32;
+            long long k_row = __shfl_sync(0xffffffffu, k_at[0], source), v_row = __shfl_sync(0xffffffffu, v_at[0], source);
+            if (LOOKS > 1) {
+                const long long k_other = __shfl_sync(0xffffffffu, k_at[LOOKS - 1], source), v_other = __shfl_sync(0xffffffffu, v_at[LOOKS - 1], source);
+                if (second) k_row = k_other, v_row = v_other;
+            }
+            if (token0 + row < ahead.span.begin || token0 + row >= ahead.span.end) k_row = -1;
             const uint32_t k_to = to + place<ROW_BYTES>(row, chunk), v_to = k_to + KEYS * ROW_BYTES;
-            if (all_known || k_row >= 0) {
-                copy16<ROW_BYTES>(k_to, k_from + k_row);
-                copy16<ROW_BYTES>(v_to, v_from + v_row);
-            } else {  // behind the length: zeros; no such page: keys of NaN
+            if (k_row >= 0) {
+                const unsigned long long in = sixteens ? row & 15 : 0;
+                copy16<ROW_BYTES>(k_to, k_from + k_row + in * k_step);
+                copy16<ROW_BYTES>(v_to, v_from + v_row + in * v_step);
+            } else {  // not attended: zeros; no such page: keys of NaN
                 fill16(k_to, k_row == -1 ? 0u : Cfg::CODES ? 0x7f7f7f7fu : 0x7fff7fffu);
                 fill16(v_to, 0u);
             }
@@ -322,30 +354,40 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     // (and a scale that underflows stays above 0: a masked score is -inf and not -inf * 0)
     const float scale = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * LOG2E * (Cfg::CODES ? a.cache.k_scale : 1.f), 1.2e-38f);
     const uint32_t turn = a.scale < 0.f ? 0x80008000u : 0u;
-    const auto begin_head = [&]() {
+    // the query rows of the head that comes next: loaded before the last one's parts are merged, used behind that (behind it
+    // where the registers would not hold both)
+    constexpr bool EARLY = !Cfg::CODES || DIM * HT <= 128;
+    uint2 raw[Cfg::CODES ? HT : 1][Cfg::CODES ? DT : 1];
+    const auto load_queries = [&]() {
         const int kv = now.head / heads.groups, row0 = (now.head % heads.groups) * Cfg::ROWS;
 #pragma unroll
         for (int m = 0; m < HT; ++m) {
             const int row = row0 + m * 8 + g;
             const T* from = static_cast<const T*>(a.q) + now.b * a.q_stride[0] + (static_cast<long long>(kv) * heads.group + row) * a.q_stride[1];
             const bool real = row < heads.group && a.scale != 0.f;
-            float mine = scale;
-            if (!Cfg::CODES) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
+            for (int d = 0; d < DT; ++d) {
+                if (Cfg::CODES) {
+                    raw[m][d] = real ? *reinterpret_cast<const uint2*>(from + d * 16 + quad * 4) : make_uint2(0u, 0u);
+                } else {
                     q[m][d][0] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + quad * 2) ^ turn : 0u;
                     q[m][d][1] = real ? *reinterpret_cast<const uint32_t*>(from + d * 16 + 8 + quad * 2) ^ turn : 0u;
                 }
-            } else {
+            }
+        }
+    };
+    const auto begin_head = [&]() {
+#pragma unroll
+        for (int m = 0; m < HT; ++m) {
+            float mine = scale;
+            if (Cfg::CODES) {
                 // an e4m3 row's dims 4 quad .. 4 quad + 3 come in one word, so the query's dims are dealt the same way. The
                 // product is of f16: a bf16 query's row is first scaled by a power of two to 1 <= max < 2, so that it fits
                 // (what falls below 2^-24 of the row's maximum is rounded away, far below the query's own 2^-8 steps)
-                uint2 raw[DT];
                 float most = 0.f;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    raw[d] = real ? *reinterpret_cast<const uint2*>(from + d * 16 + quad * 4) : make_uint2(0u, 0u);
-                    const T* x = reinterpret_cast<const T*>(&raw[d]);
+                    const T* x = reinterpret_cast<const T*>(&raw[m][d]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(to_f32(x[e])));
                 }
@@ -357,7 +399,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                 mine = fmaxf(scale * __int_as_float((127 + power) << 23), 1.2e-38f);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const T* x = reinterpret_cast<const T*>(&raw[d]);
+                    const T* x = reinterpret_cast<const T*>(&raw[m][d]);
                     q[m][d][0] = frag::pack_f32<false>(to_f32(x[0]) * down, to_f32(x[1]) * down) ^ turn;
                     q[m][d][1] = frag::pack_f32<false>(to_f32(x[2]) * down, to_f32(x[3]) * down) ^ turn;
                 }
@@ -376,8 +418,8 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
 
     float* const merge = reinterpret_cast<float*>(smem + WARPS * STAGES * Cfg::STEP_BYTES);
     // the warps' maxima, sums and outputs of a head become one, eight query heads at a time; whole heads go out, cut ones to a piece
-    const auto end_head = [&](float* piece) {
-        const int kv = now.head / heads.groups, row0 = (now.head % heads.groups) * Cfg::ROWS;
+    const auto end_head = [&](int b, int head, float* piece) {
+        const int kv = head / heads.groups, row0 = (head % heads.groups) * Cfg::ROWS;
         const int rows = min(Cfg::ROWS, heads.group - row0);
 #pragma unroll
         for (int m = 0; m < HT; ++m) {
@@ -422,13 +464,14 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                     *reinterpret_cast<float4*>(to + d) = acc;
                     if (d == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(best, s);
                 } else {
-                    put_out<Cfg, T>(a, now.b, static_cast<long long>(kv) * heads.group + row0 + row, d, acc, best, s);
+                    put_out<Cfg, T>(a, b, static_cast<long long>(kv) * heads.group + row0 + row, d, acc, best, s);
                 }
             }
             }
         }
     };
 
+    load_queries();
     begin_head();
     int stage = 0;
     bool cut_in_front = now.t > 0;  // the head's tiles before these belong to an earlier CTA
@@ -439,7 +482,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
         feed(stage == 0 ? STAGES - 1 : stage - 1);
         const uint32_t from = ring + stage * Cfg::STEP_BYTES;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
-        const uint32_t token0 = now.span.begin + now.t * Cfg::TILE + warp * KEYS;
+        const uint32_t token0 = (now.span.begin & ~15u) + now.t * Cfg::TILE + warp * KEYS;
         if (token0 < now.span.end) {
             // ---- scores
             constexpr int CHAINS = HT * KT >= 4 ? 1 : 2;  // sums that a score is made of: products of one sum wait for one another
@@ -486,12 +529,12 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[m][j][e] += s2[m][j][e];
             }
-            if (token0 + KEYS > now.span.end) {
+            if (token0 < now.span.begin || token0 + KEYS > now.span.end) {
 #pragma unroll
                 for (int j = 0; j < KT; ++j)
 #pragma unroll
                     for (int half = 0; half < 2; ++half)
-                        if (token0 + j * 16 + half * 8 + g >= now.span.end) {
+                        if (token0 + j * 16 + half * 8 + g < now.span.begin || token0 + j * 16 + half * 8 + g >= now.span.end) {
 #pragma unroll
                             for (int m = 0; m < HT; ++m) s[m][j][half * 2] = s[m][j][half * 2 + 1] = -INFINITY;
                         }
@@ -572,19 +615,28 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
 
         // ---- the end of a head, or of the share
         const bool head_ends = now.t + 1 == now.tiles, share_ends = step + 1 == steps;
+        const int b = now.b, head = now.head;
         if (head_ends || share_ends) {
             float* piece = nullptr;
             if (cut_in_front || !head_ends) piece = pieces + (2ll * blockIdx.x + (cut_in_front ? 0 : 1)) * (Cfg::ROWS * Cfg::PITCH);
-            end_head(piece);
             if (!head_ends && !cut_in_front) {  // the head starts here and goes on: the CTAs up to the one that holds its last tile
                 const long long last = x1 - 1 + (now.tiles - 1 - now.t);
-                record = {now.b, now.head, static_cast<int>(blockIdx.x), static_cast<int>(((last + 1) * n + all - 1) / all - 1 - blockIdx.x + 1)};
+                record = {b, head, static_cast<int>(blockIdx.x), static_cast<int>(((last + 1) * n + all - 1) / all - 1 - blockIdx.x + 1)};
             }
-            if (by_head && tid == 0 && !cut_in_front) records[now.b * heads.cut + now.head] = head_ends ? Record{0, 0, 0, 0} : record;
+            if (by_head && tid == 0 && !cut_in_front) records[b * heads.cut + head] = head_ends ? Record{0, 0, 0, 0} : record;
             cut_in_front = false;
+            if (!share_ends) {
+                advance<Cfg>(now, a, heads.cut);
+                if (EARLY) load_queries();
+            }
+            end_head(b, head, piece);
+            if (!share_ends) {
+                if (!EARLY) load_queries();
+                begin_head();
+            }
+        } else {
+            ++now.t;
         }
-        advance<Cfg>(now, a, heads.cut);
-        if (head_ends && !share_ends) begin_head();
     }
     if (tid == 0 && records && !by_head) records[blockIdx.x] = record;
 }
@@ -663,10 +715,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_p
 
 template <class Cfg> int64_t piece_bytes() { return 2ll * Cfg::ROWS * Cfg::PITCH * 4; }
 
-// no request has more keys (one without a page among them where a length is beyond its table row)
+// no request's tiles cover more keys (one without a page among them where a length is beyond its table row, and up to 15
+// before a window)
 int64_t longest_of(const emb_paged_attend_t& a) {
     const int64_t most = static_cast<int64_t>(a.table_width) * a.cache.page_size + 1;
-    return a.window ? std::min<int64_t>(a.window, most) : most;
+    return a.window ? std::min<int64_t>(a.window + 15ll, most) : most;
 }
 
 // the CTAs of a launch: as many as the SMs hold at once, or as there can be tiles
@@ -697,7 +750,7 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     cudaGetDevice(&device);
     std::call_once(once[device], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM); });
     Record* records = cuts ? static_cast<Record*>(a.workspace) : nullptr;
-    float* pieces = reinterpret_cast<float*>(records + grid);
+    float* pieces = cuts ? reinterpret_cast<float*>(records + grid) : nullptr;
     if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), Cfg::THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), records, by_head, pieces))) return r;
     if (!cuts) return 0;
     // about four CTAs an SM where records are few, each with as many warps for a row as its rows leave

@@ -347,7 +347,7 @@ def test_attend_pages(paged, size, layout, cache):
     check_attend(paged, s)
 
 
-@pytest.mark.parametrize("window", [1, 16, 63, 64, 65, 1000])
+@pytest.mark.parametrize("window", [1, 16, 48, 49, 50, 63, 64, 65, 113, 240, 241, 256, 257, 1000])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_attend_window(paged, window, dim):
     check_attend(paged, make_attend([1, 64, 65, 500, 0, 1200, 2000], 8, 2, dim, BF16, BF16, 16), window=window)
