@@ -12,19 +12,22 @@
 // tensor work here is a tenth of what the legacy path does in the time HBM needs for the bytes. A WARP owns KEYS
 // consecutive keys at a time: it copies them into a ring of its own with cp.async (rows found through the page table, so any
 // page size and any strides; rows behind the length are filled with zeros and not read), multiplies, and keeps a maximum,
-// sum and output of its own. Warps meet only at the end of a request's head, so no barrier stands between copies and products.
+// sum and output of its own. No barrier stands between copies and products.
+// The warps of a CTA either take the keys of one head in turn (a tile is WARPS * KEYS keys), and meet at the head's end, or,
+// where there is enough work and the number of heads allows, stand SIDE BY SIDE on neighbouring heads (a tile is KEYS keys of
+// each): then no warp waits for another, and a token's rows of several heads are read at about the same time.
 // The maximum that weights refer to moves only when a score passes it by more than 8 (a weight is at most 2^8, in f16 and f32
 // alike far from overflow): most steps then need neither the reduction over lanes nor the rescaling.
 //
-// The work is cut by TILES of WARPS * KEYS keys, all requests and heads behind one another: CTA c of n takes tiles
-// [c T / n, (c + 1) T / n), whatever their requests. So a single long request and a ragged batch both spread evenly, and
+// The work is cut by TILES, all requests and heads (or sets of heads side by side) behind one another: CTA c of n takes
+// tiles [c T / n, (c + 1) T / n), whatever their requests. So a single long request and a ragged batch both spread evenly, and
 // a request's head is cut only where a CTA's share ends. Those pieces (maximum, sum, unscaled output; two per CTA at
 // most) go to the workspace, and paged_join_kernel adds them up in the order of the keys.
 
 #include "paged_common.cuh"
 
 #include <algorithm>
-#include <mutex>
+#include <atomic>
 
 #include "emb_frag.cuh"
 
@@ -36,6 +39,10 @@ namespace frag = emb::frag;
 // Where there are no more tiles than CTAs, a request's head of at most so many tiles is not cut: on a machine that is not
 // full a CTA takes about half a microsecond for a tile more, and the join two.
 constexpr int WHOLE_TILES = 4;
+// Warps stand side by side where there are at least SIDE_SETS sets of heads for every 100 CTAs (a head is then spread over
+// few CTAs, and the join is short) and a CTA gets at least SIDE_TILES tiles (below, the latency of a head's keys one after
+// another counts, and they are better shared by the warps).
+constexpr int SIDE_SETS = 12, SIDE_TILES = 8;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 constexpr float LOWEST = -3.402823466e38f;  // seed of a maximum: finite, so that a masked score (-inf) against it weighs 0
@@ -48,9 +55,11 @@ template <class T, class C, int DIM_, int HT_> struct Config {
     static constexpr int ROW_BYTES = DIM * static_cast<int>(sizeof(C));
     static constexpr int KEYS = ROW_BYTES >= 256 || (ROW_BYTES == 128 && HT == 4) ? 16 : ROW_BYTES == 128 || HT == 4 ? 32 : 64;  // of a warp per step
     static constexpr int STEP_BYTES = 2 * KEYS * ROW_BYTES;                         // keys, then values
-    static constexpr int WARPS = ROW_BYTES == 512 ? 3 : 4, THREADS = WARPS * 32;
-    static constexpr int CTAS = DIM * HT > 256 || ROW_BYTES == 512 ? 2 : 3;  // per SM
-    static constexpr int TILE = WARPS * KEYS;
+    static constexpr int WARPS = ROW_BYTES == 512 ? 2 : 4, THREADS = WARPS * 32;
+    static constexpr int CTAS = HT == 4 || (DIM * HT > 256 && ROW_BYTES < 512) ? 2 : 3;  // per SM
+    static constexpr int TILE = WARPS * KEYS;                                       // where the warps share a head
+    static constexpr int TILE_SHIFT = (KEYS == 64 ? 6 : KEYS == 32 ? 5 : 4) + (WARPS == 4 ? 2 : 1);
+    static_assert(TILE == 1 << TILE_SHIFT, "a power of two");
     static constexpr int PITCH = DIM + 4;         // floats of a row of a piece: outputs, maximum, sum
     static constexpr int MERGED = 512 / DIM;      // query heads whose parts the warps merge at a time
     static constexpr int MERGE_BYTES = WARPS * MERGED * PITCH * 4;
@@ -60,11 +69,18 @@ template <class T, class C, int DIM_, int HT_> struct Config {
     static_assert(CTAS * (SMEM + 1024 + 128) <= 228 * 1024, "shared memory of an SM");
 };
 
-// A head that was cut: the CTA that holds its first tiles and how many hold one (0: nothing to join). A CTA has two places
-// for pieces: the head that an earlier CTA began, and the head that goes on in later ones. A list has one record for each
-// CTA (of the head that goes on), or one for each head where there are fewer heads than CTAs.
+// A head that was cut: the CTA that holds its first tiles, how many hold one (0: nothing to join), and the warp's place
+// beside the others. A CTA has two places for pieces for each warp: of the head that an earlier CTA began, and of the head
+// that goes on in later ones. A list has `side` records for each CTA (of the heads that go on), or one for each head where
+// those are fewer.
 struct Record {
-    int32_t request, head, cta, pieces;
+    int32_t request, head, cta, pieces, slot, unused[3];
+};
+struct Places {  // of records and pieces
+    Record* records;
+    float* pieces;  // null: no head is cut
+    int32_t by_head, side, floats;  // heads side by side at most; floats of a piece
+    __device__ __forceinline__ float* piece(long long cta, int second, int slot) const { return pieces + ((2 * cta + second) * side + slot) * floats; }
 };
 
 struct Heads {  // how query heads fall on the rows of a CTA
@@ -88,23 +104,24 @@ __device__ __forceinline__ Span span_of(const emb_paged_attend_t& a, int b) {
 }
 
 // tiles begin at a multiple of 16 keys, at or before the first one
-template <int TILE> __device__ __forceinline__ uint32_t tiles_of(const Span& s) { return max(1u, (s.end - (s.begin & ~15u) + TILE - 1) / TILE); }
+__device__ __forceinline__ uint32_t tiles_of(const Span& s, int shift) { return max(1u, (s.end - (s.begin & ~15u) + (1u << shift) - 1) >> shift); }
 
 struct Cursor {  // a tile of the CTA's share
-    int b, head;
+    int b, set;  // heads side by side: set * side + the warp's place
     uint32_t t, tiles;
     Span span;
 };
 
-template <class Cfg> __device__ __forceinline__ void advance(Cursor& c, const emb_paged_attend_t& a, int cut) {
+__device__ __forceinline__ void advance(Cursor& c, const emb_paged_attend_t& a, int sets, int shift) {
     if (++c.t < c.tiles) return;
     c.t = 0;
-    if (++c.head < cut) return;
-    c.head = 0;
+    if (++c.set < sets) return;
+    c.set = 0;
     if (++c.b >= a.requests) return;
     c.span = span_of(a, c.b);
-    c.tiles = tiles_of<Cfg::TILE>(c.span);
+    c.tiles = tiles_of(c.span, shift);
 }
+
 
 // A copy brings 128 bytes into L2 unless it says otherwise. A row of 64 bytes (64 e4m3 codes) of a token-major cache has
 // another head's row beside it, read at another time: 64 bytes of each 128 were fetched at 3.4 TB/s of useful bytes
@@ -150,13 +167,17 @@ __device__ __forceinline__ void add_part(float4& acc, float& s, const float4& x,
     s += f * sum;
 }
 
-// four dims of a finished row: rounded once; a row without keys is 0
+// what a finished row's sum of weighted values is multiplied with; a row without keys is 0
+template <class Cfg> __device__ __forceinline__ float share_of(const emb_paged_attend_t& a, float s) { return s == 0.f ? 0.f : (Cfg::CODES ? a.cache.v_scale : 1.f) / s; }
+__device__ __forceinline__ float log_sum(float top, float s) { return s == 0.f ? -INFINITY : top * LN2 + logf(s); }
+
+// four dims of a finished row, rounded once
 template <class Cfg, class T> __device__ __forceinline__ void put_out(const emb_paged_attend_t& a, int b, long long h, int d, const float4& acc, float best, float s) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    const float inv = s == 0.f ? 0.f : (Cfg::CODES ? a.cache.v_scale : 1.f) / s;
+    const float inv = share_of<Cfg>(a, s);
     const uint2 packed = make_uint2(frag::pack_f32<BF16>(acc.x * inv, acc.y * inv), frag::pack_f32<BF16>(acc.z * inv, acc.w * inv));
     *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[1] + d) = packed;
-    if (a.lse && d == 0) a.lse[b * static_cast<long long>(a.heads) + h] = s == 0.f ? -INFINITY : best * LN2 + logf(s);
+    if (a.lse && d == 0) a.lse[b * static_cast<long long>(a.heads) + h] = log_sum(best, s);
 }
 
 // P^T of eight keys: from rows of keys (a lane: key g, heads 2 quad, 2 quad + 1) to the operand (keys 2 quad, 2 quad + 1, head g)
@@ -167,82 +188,94 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 
 template <class T, class C, int DIM, int HT>
-__global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C, DIM, HT>::CTAS)) paged_attend_kernel(const emb_paged_attend_t a, const Divisor page_size, Record* __restrict__ records, bool by_head, float* __restrict__ pieces) {
+__global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C, DIM, HT>::CTAS)) paged_attend_kernel(const __grid_constant__ emb_paged_attend_t a, const Divisor page_size, const Places places) {
     using Cfg = Config<T, C, DIM, HT>;
     constexpr int WARPS = Cfg::WARPS, THREADS = Cfg::THREADS, KEYS = Cfg::KEYS, KT = KEYS / 16, DT = DIM / 16, ROW_BYTES = Cfg::ROW_BYTES, STAGES = Cfg::STAGES;
     constexpr int LOOKS = (KEYS + 31) / 32;  // keys that a lane looks up per step, at most
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ long long scan_slab[WARPS], share[2];
+    __shared__ long long scan_slab[2][WARPS], share[2];
     __shared__ long long first_before;  // tiles before the request that holds the share's first tile
-    __shared__ int first_request;
+    __shared__ int first_request, holders;  // holders: CTAs from this one on that hold tiles of the head its share ends in
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, quad = lane & 3;
     follow_on();
     const Heads heads(a, Cfg::ROWS);
+    const bool lists = places.pieces && !places.by_head;  // this CTA owes `side` records
 
-    // ---- the CTA's share of the tiles
-    const auto scan = [&](int base, uint32_t& tiles, long long& total) -> long long {  // tiles up to and with request base + tid
-        tiles = base + tid < a.requests ? tiles_of<Cfg::TILE>(span_of(a, base + tid)) : 0u;
-        long long v = static_cast<long long>(tiles) * heads.cut;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, v, d);
-            if (lane >= d) v += x;
-        }
-        __syncthreads();
-        if (lane == 31) scan_slab[warp] = v;
-        __syncthreads();
-        total = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) v += scan_slab[w];
-            total += scan_slab[w];
-        }
-        return v;
-    };
-    long long all = 0, chunk_total;
-    uint32_t tiles;
-    long long upto = 0;
-    for (int base = 0; base < a.requests; base += THREADS) {
-        upto = scan(base, tiles, chunk_total) + all;
-        all += chunk_total;
+    // ---- how the warps stand, and the CTA's share of the tiles
+    const int side_shift = Cfg::TILE_SHIFT - (places.side >= 4 ? 2 : places.side >= 2 ? 1 : 0);
+    long long in_turn = 0, beside = 0;
+    for (int b = tid; b < a.requests; b += THREADS) {
+        const Span s = span_of(a, b);
+        in_turn += static_cast<long long>(tiles_of(s, Cfg::TILE_SHIFT)) * heads.cut;
+        beside += static_cast<long long>(tiles_of(s, side_shift)) * (heads.cut / places.side);
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) in_turn += __shfl_xor_sync(0xffffffffu, in_turn, d), beside += __shfl_xor_sync(0xffffffffu, beside, d);
+    if (lane == 0) scan_slab[0][warp] = in_turn, scan_slab[1][warp] = beside;
+    __syncthreads();
+    in_turn = beside = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) in_turn += scan_slab[0][w], beside += scan_slab[1][w];
+    const bool stand = beside >= static_cast<long long>(SIDE_TILES) * gridDim.x && static_cast<long long>(a.requests) * (heads.cut / places.side) * 100 >= SIDE_SETS * static_cast<long long>(gridDim.x);
+    const int side = stand ? places.side : 1;
+    const int sharing = WARPS / side;  // warps on one head
+    const int shift = side > 1 ? side_shift : Cfg::TILE_SHIFT, sets = heads.cut / side;
+    const int slot = warp / sharing, turn_of = warp % sharing;  // the warp's head in a set, and its turn among those on it
+    const long long all = side > 1 ? beside : in_turn;
     const long long n = min(static_cast<long long>(gridDim.x), all);
     if (static_cast<long long>(blockIdx.x) >= n) {
-        if (tid == 0 && records && !by_head) records[blockIdx.x].pieces = 0;
+        if (tid < places.side && lists) places.records[blockIdx.x * places.side + tid].pieces = 0;
         return;
     }
-    const uint32_t whole = !pieces ? 0xffffffffu : all <= static_cast<long long>(gridDim.x) ? WHOLE_TILES : 0;  // no place for pieces: no cuts
+    const uint32_t whole = !places.pieces ? 0xffffffffu : all <= static_cast<long long>(gridDim.x) ? WHOLE_TILES : 0;  // no place for pieces: no cuts
     if (tid < 2) share[tid] = all * (blockIdx.x + tid) / n;
+    if (tid == 0) holders = 0;
     __syncthreads();
     const long long want0 = share[0], want1 = share[1];
-    __syncthreads();
     long long before_chunk = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
-        if (a.requests > THREADS) {
-            upto = scan(base, tiles, chunk_total) + before_chunk;
-            before_chunk += chunk_total;
+        const uint32_t tiles = base + tid < a.requests ? tiles_of(span_of(a, base + tid), shift) : 0u;
+        long long upto = static_cast<long long>(tiles) * sets;  // tiles up to and with request base + tid
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
         }
-        const long long from = upto - static_cast<long long>(tiles) * heads.cut;
+        __syncthreads();  // the slab's last readers are done, and `share` is read
+        if (lane == 31) scan_slab[0][warp] = upto;
+        __syncthreads();
+        upto += before_chunk;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) upto += scan_slab[0][w];
+            before_chunk += scan_slab[0][w];
+        }
+        const long long from = upto - static_cast<long long>(tiles) * sets;
         // a border inside a head that is not to be cut moves to the head's first tile
         if (from <= want0 && want0 < upto) {
             const long long x = tiles <= whole ? from + (want0 - from) / tiles * tiles : want0;
             share[0] = x, first_request = base + tid, first_before = from;
         }
-        if (from <= want1 && want1 < upto && tiles <= whole) share[1] = from + (want1 - from) / tiles * tiles;
+        if (from <= want1 && want1 < upto) {
+            const long long head_from = from + (want1 - from) / tiles * tiles;
+            if (tiles <= whole) share[1] = head_from;
+            else if (head_from < want1) holders = static_cast<int>(((head_from + tiles) * n + all - 1) / all - blockIdx.x);
+        }
     }
     __syncthreads();
     const long long x0 = share[0], x1 = share[1];
     if (x0 >= x1) {
-        if (tid == 0 && records && !by_head) records[blockIdx.x].pieces = 0;
+        if (tid < places.side && lists) places.records[blockIdx.x * places.side + tid].pieces = 0;
         return;
     }
     Cursor ahead;
     ahead.b = first_request;
     ahead.span = span_of(a, ahead.b);
-    ahead.tiles = tiles_of<Cfg::TILE>(ahead.span);
-    ahead.head = static_cast<int>((x0 - first_before) / ahead.tiles);
+    ahead.tiles = tiles_of(ahead.span, shift);
+    ahead.set = static_cast<int>((x0 - first_before) / ahead.tiles);
     ahead.t = static_cast<uint32_t>((x0 - first_before) % ahead.tiles);
     Cursor now = ahead;
+    const auto token_at = [&](const Cursor& c) { return (c.span.begin & ~15u) + (c.t << shift) + turn_of * KEYS; };  // the warp's first
 
     // ---- copies: a lane finds a key's row, the warp copies KEYS of them
     const uint32_t ring = frag::smem_addr(smem) + warp * (STAGES * Cfg::STEP_BYTES);
@@ -253,7 +286,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     // time, else one
     const bool sixteens = page_size.d % 16 == 0;
     const auto token_of = [&](int look) {
-        return (ahead.span.begin & ~15u) + ahead.t * Cfg::TILE + warp * KEYS + (sixteens ? lane % (KEYS / 16) * 16 : look * 32 + lane % min(KEYS, 32));
+        return token_at(ahead) + (sixteens ? lane % (KEYS / 16) * 16 : look * 32 + lane % min(KEYS, 32));
     };
     // found a step before they are needed: the page id (-1: behind the length, -2: none) and the token in it
     int page[LOOKS];
@@ -277,7 +310,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     const char* const k_from = static_cast<const char*>(a.cache.k) + chunk * 16;
     const char* const v_from = static_cast<const char*>(a.cache.v) + chunk * 16;
     const auto issue = [&](int stage) {
-        const uint32_t kv = ahead.head / heads.groups;
+        const uint32_t kv = (ahead.set * side + slot) / heads.groups;
         // byte offsets of the rows (strides are below 2^32 elements), or the page id where there is no row
         long long k_at[LOOKS], v_at[LOOKS];
         bool known = true;
@@ -292,7 +325,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
             known = known && one;
         }
         const uint32_t to = ring + stage * Cfg::STEP_BYTES;
-        const uint32_t token0 = (ahead.span.begin & ~15u) + ahead.t * Cfg::TILE + warp * KEYS;
+        const uint32_t token0 = token_at(ahead);
         if (sixteens && __all_sync(0xffffffffu, known) && token0 >= ahead.span.begin && token0 + KEYS <= ahead.span.end) {
 #pragma unroll
             for (int s = 0; s < KEYS / 16; ++s) {
@@ -332,13 +365,13 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
         }
     };
 
-    const long long steps = x1 - x0;
-    long long issued = 0;
+    const uint32_t steps = static_cast<uint32_t>(x1 - x0);
+    uint32_t issued = 0;
     find_pages();
     const auto feed = [&](int stage) {
         if (issued < steps) {
             issue(stage);
-            advance<Cfg>(ahead, a, heads.cut);
+            advance(ahead, a, sets, shift);
             if (issued + 1 < steps) find_pages();
         }
         ++issued;
@@ -359,7 +392,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     constexpr bool EARLY = !Cfg::CODES || DIM * HT <= 128;
     uint2 raw[Cfg::CODES ? HT : 1][Cfg::CODES ? DT : 1];
     const auto load_queries = [&]() {
-        const int kv = now.head / heads.groups, row0 = (now.head % heads.groups) * Cfg::ROWS;
+        const int head = now.set * side + slot, kv = head / heads.groups, row0 = (head % heads.groups) * Cfg::ROWS;
 #pragma unroll
         for (int m = 0; m < HT; ++m) {
             const int row = row0 + m * 8 + g;
@@ -417,56 +450,103 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     };
 
     float* const merge = reinterpret_cast<float*>(smem + WARPS * STAGES * Cfg::STEP_BYTES);
-    // the warps' maxima, sums and outputs of a head become one, eight query heads at a time; whole heads go out, cut ones to a piece
-    const auto end_head = [&](int b, int head, float* piece) {
+    const auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(sharing * 32) : "memory"); };  // of the warps on one head
+    // the sums of heads 2 quad and 2 quad + 1 over the lanes' keys
+    const auto sums_of = [&](int m, float (&sum)[2]) {
+        sum[0] = total[m][0], sum[1] = total[m][1];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
+    };
+    const auto put_part = [&](int m, int e, float sum, float* to) {  // a row's outputs, maximum and sum
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            if (Cfg::CODES) *reinterpret_cast<float2*>(to + d * 16 + g * 2) = make_float2(o[m][d][e], o[m][d][e + 2]);
+            else to[d * 16 + g] = o[m][d][e], to[d * 16 + g + 8] = o[m][d][e + 2];
+        }
+        if (g == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(top[m][e], sum);
+    };
+    // a head that the warp has alone: out, or to its piece
+    const auto end_alone = [&](int b, int head, float* piece) {
         const int kv = head / heads.groups, row0 = (head % heads.groups) * Cfg::ROWS;
         const int rows = min(Cfg::ROWS, heads.group - row0);
 #pragma unroll
         for (int m = 0; m < HT; ++m) {
             if (m * 8 >= rows) break;
-            float sum[2] = {total[m][0], total[m][1]};
+            float sum[2], inv[2];
+            sums_of(m, sum);
+            if (piece) {
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
-#pragma unroll
-            for (int first = 0; first < 8; first += Cfg::MERGED) {
-            if (m * 8 + first >= rows) break;
-            __syncthreads();  // the last heads are read
+                for (int e = 0; e < 2; ++e)
+                    if (m * 8 + quad * 2 + e < rows) put_part(m, e, sum[e], piece + (m * 8 + quad * 2 + e) * Cfg::PITCH);
+                continue;
+            }
+            const long long h0 = static_cast<long long>(kv) * heads.group + row0 + m * 8;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int r = quad * 2 + e - first;
-                if (r < 0 || r >= Cfg::MERGED || m * 8 + first + r >= rows) continue;
-                float* to = merge + (warp * Cfg::MERGED + r) * Cfg::PITCH;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    if (Cfg::CODES) *reinterpret_cast<float2*>(to + d * 16 + g * 2) = make_float2(o[m][d][e], o[m][d][e + 2]);
-                    else to[d * 16 + g] = o[m][d][e], to[d * 16 + g + 8] = o[m][d][e + 2];
-                }
-                if (g == 0) to[DIM] = top[m][e], to[DIM + 1] = sum[e];
+                inv[e] = share_of<Cfg>(a, sum[e]);
+                if (a.lse && g == 0 && m * 8 + quad * 2 + e < rows) a.lse[b * static_cast<long long>(a.heads) + h0 + quad * 2 + e] = log_sum(top[m][e], sum[e]);
             }
-            __syncthreads();
-            for (int i = tid; i < Cfg::MERGED * (DIM / 4); i += THREADS) {
-                const int r = i / (DIM / 4), d = i % (DIM / 4) * 4, row = m * 8 + first + r;
-                if (row >= rows) break;
-                float best = LOWEST;
+            T* const to = static_cast<T*>(a.out) + b * a.out_stride[0] + (h0 + g) * a.out_stride[1];
+            constexpr bool OUT_BF16 = std::is_same<T, __nv_bfloat16>::value;
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) best = fmaxf(best, merge[(w * Cfg::MERGED + r) * Cfg::PITCH + DIM]);
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                float s = 0.f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float* from = merge + (w * Cfg::MERGED + r) * Cfg::PITCH;
-                    add_part(acc, s, *reinterpret_cast<const float4*>(from + d), exp2_(from[DIM] - best), from[DIM + 1]);
-                }
-                if (piece) {
-                    float* to = piece + row * Cfg::PITCH;
-                    *reinterpret_cast<float4*>(to + d) = acc;
-                    if (d == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(best, s);
+            for (int d = 0; d < DT; ++d) {  // turned: a lane has dims of head g
+                const uint32_t x = transposed(frag::pack_f32<OUT_BF16>(o[m][d][0] * inv[0], o[m][d][1] * inv[1]));
+                const uint32_t y = transposed(frag::pack_f32<OUT_BF16>(o[m][d][2] * inv[0], o[m][d][3] * inv[1]));
+                if (m * 8 + g >= rows) continue;
+                if (Cfg::CODES) {  // x: dims 4 quad and 4 quad + 2, y: 4 quad + 1 and 4 quad + 3
+                    *reinterpret_cast<uint2*>(to + d * 16 + quad * 4) = make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
                 } else {
-                    put_out<Cfg, T>(a, b, static_cast<long long>(kv) * heads.group + row0 + row, d, acc, best, s);
+                    *reinterpret_cast<uint32_t*>(to + d * 16 + quad * 2) = x;
+                    *reinterpret_cast<uint32_t*>(to + d * 16 + 8 + quad * 2) = y;
                 }
             }
+        }
+    };
+    // one that warps share: their maxima, sums and outputs become one, MERGED query heads at a time
+    const auto end_shared = [&](int b, int head, float* piece) {
+        const int kv = head / heads.groups, row0 = (head % heads.groups) * Cfg::ROWS;
+        const int rows = min(Cfg::ROWS, heads.group - row0);
+#pragma unroll
+        for (int m = 0; m < HT; ++m) {
+            if (m * 8 >= rows) break;
+            float sum[2];
+            sums_of(m, sum);
+#pragma unroll
+            for (int first = 0; first < 8; first += Cfg::MERGED) {
+                if (m * 8 + first >= rows) break;
+                meet();  // the last heads are read
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = quad * 2 + e - first;
+                    if (r >= 0 && r < Cfg::MERGED && m * 8 + first + r < rows) put_part(m, e, sum[e], merge + (warp * Cfg::MERGED + r) * Cfg::PITCH);
+                }
+                meet();
+                const float* const parts = merge + slot * sharing * Cfg::MERGED * Cfg::PITCH;
+                for (int i = turn_of * 32 + lane; i < Cfg::MERGED * (DIM / 4); i += sharing * 32) {
+                    const int r = i / (DIM / 4), d = i % (DIM / 4) * 4, row = m * 8 + first + r;
+                    if (row >= rows) break;
+                    float best = LOWEST;
+#pragma unroll
+                    for (int w = 0; w < WARPS; ++w)
+                        if (w < sharing) best = fmaxf(best, parts[(w * Cfg::MERGED + r) * Cfg::PITCH + DIM]);
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float s = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WARPS; ++w) {
+                        if (w >= sharing) break;
+                        const float* from = parts + (w * Cfg::MERGED + r) * Cfg::PITCH;
+                        add_part(acc, s, *reinterpret_cast<const float4*>(from + d), exp2_(from[DIM] - best), from[DIM + 1]);
+                    }
+                    if (piece) {
+                        float* to = piece + row * Cfg::PITCH;
+                        *reinterpret_cast<float4*>(to + d) = acc;
+                        if (d == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(best, s);
+                    } else {
+                        put_out<Cfg, T>(a, b, static_cast<long long>(kv) * heads.group + row0 + row, d, acc, best, s);
+                    }
+                }
             }
         }
     };
@@ -475,14 +555,14 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     begin_head();
     int stage = 0;
     bool cut_in_front = now.t > 0;  // the head's tiles before these belong to an earlier CTA
-    Record record{0, 0, 0, 0};  // of the head that goes on
-    for (long long step = 0; step < steps; ++step) {
+    Record record{};  // of the head that goes on
+    for (uint32_t step = 0; step < steps; ++step) {
         frag::cp_async_wait<STAGES - 2>();
         __syncwarp();
         feed(stage == 0 ? STAGES - 1 : stage - 1);
         const uint32_t from = ring + stage * Cfg::STEP_BYTES;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
-        const uint32_t token0 = (now.span.begin & ~15u) + now.t * Cfg::TILE + warp * KEYS;
+        const uint32_t token0 = token_at(now);
         if (token0 < now.span.end) {
             // ---- scores
             constexpr int CHAINS = HT * KT >= 4 ? 1 : 2;  // sums that a score is made of: products of one sum wait for one another
@@ -615,21 +695,19 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
 
         // ---- the end of a head, or of the share
         const bool head_ends = now.t + 1 == now.tiles, share_ends = step + 1 == steps;
-        const int b = now.b, head = now.head;
+        const int b = now.b, head = now.set * side + slot;
         if (head_ends || share_ends) {
             float* piece = nullptr;
-            if (cut_in_front || !head_ends) piece = pieces + (2ll * blockIdx.x + (cut_in_front ? 0 : 1)) * (Cfg::ROWS * Cfg::PITCH);
-            if (!head_ends && !cut_in_front) {  // the head starts here and goes on: the CTAs up to the one that holds its last tile
-                const long long last = x1 - 1 + (now.tiles - 1 - now.t);
-                record = {b, head, static_cast<int>(blockIdx.x), static_cast<int>(((last + 1) * n + all - 1) / all - 1 - blockIdx.x + 1)};
-            }
-            if (by_head && tid == 0 && !cut_in_front) records[b * heads.cut + head] = head_ends ? Record{0, 0, 0, 0} : record;
+            if (cut_in_front || !head_ends) piece = places.piece(blockIdx.x, !cut_in_front, slot);
+            if (!head_ends && !cut_in_front) record = {b, head, static_cast<int>(blockIdx.x), holders, slot, {}};  // it starts here and goes on
+            if (places.by_head && turn_of == 0 && lane == 0 && !cut_in_front) places.records[b * heads.cut + head] = head_ends ? Record{} : record;
             cut_in_front = false;
             if (!share_ends) {
-                advance<Cfg>(now, a, heads.cut);
+                advance(now, a, sets, shift);
                 if (EARLY) load_queries();
             }
-            end_head(b, head, piece);
+            if (sharing == 1) end_alone(b, head, piece);
+            else end_shared(b, head, piece);
             if (!share_ends) {
                 if (!EARLY) load_queries();
                 begin_head();
@@ -638,7 +716,10 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
             ++now.t;
         }
     }
-    if (tid == 0 && records && !by_head) records[blockIdx.x] = record;
+    if (lists) {
+        if (turn_of == 0 && lane == 0) places.records[blockIdx.x * places.side + slot] = record;
+        if (tid >= side && tid < places.side) places.records[blockIdx.x * places.side + tid].pieces = 0;
+    }
 }
 
 // The pieces of the heads that were cut, a record and some rows of it for each CTA. A row's maximum and sum are joined as
@@ -647,12 +728,12 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
 constexpr int JOIN_WARPS = 8;
 
 template <class T, class C, int DIM, int HT>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_paged_attend_t a, const Record* records, const float* pieces, int split) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_paged_attend_t a, const Places places, int split) {
     using Cfg = Config<T, C, DIM, HT>;
     constexpr int PER_LANE = DIM / 32;
     __shared__ float slab[JOIN_WARPS][Cfg::PITCH];
     follow_on();
-    const Record record = records[blockIdx.x];
+    const Record record = places.records[blockIdx.x];
     if (record.pieces == 0) return;
     const Heads heads(a, Cfg::ROWS);
     const int kv = record.head / heads.groups, row0 = (record.head % heads.groups) * Cfg::ROWS;
@@ -660,9 +741,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_p
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % split, at_once = JOIN_WARPS / split;
     for (int base = blockIdx.y * at_once; base < rows; base += gridDim.y * at_once) {
         const int r = min(base + warp / split, rows - 1);
-        // piece i: the first in its CTA's second place, the others in their CTAs' first
-        const float* const from = pieces + 2ll * record.cta * (Cfg::ROWS * Cfg::PITCH) + r * Cfg::PITCH;
-        const auto piece = [&](int i) { return from + (2 * i + (i == 0)) * static_cast<long long>(Cfg::ROWS * Cfg::PITCH); };
+        // the first in its CTA's second place, the others in their CTAs' first
+        const auto piece = [&](int i) -> const float* { return places.piece(record.cta + i, i == 0, record.slot) + r * Cfg::PITCH; };
         float best = LOWEST;
         for (int k = lane; k < record.pieces; k += 32) best = fmaxf(best, piece(k)[DIM]);
         float acc[PER_LANE] = {}, s = 0.f;
@@ -713,8 +793,6 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_p
     }
 }
 
-template <class Cfg> int64_t piece_bytes() { return 2ll * Cfg::ROWS * Cfg::PITCH * 4; }
-
 // no request's tiles cover more keys (one without a page among them where a length is beyond its table row, and up to 15
 // before a window)
 int64_t longest_of(const emb_paged_attend_t& a) {
@@ -735,9 +813,14 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     if (!sms) return refuse("paged_attend: the current device cannot be asked for its SMs");
     const int grid = grid_of<Cfg>(a, sms);
     const bool cuts = grid == sms * Cfg::CTAS || longest_of(a) > WHOLE_TILES * Cfg::TILE;  // else no head is cut
-    const int64_t cut_heads = static_cast<int64_t>(a.requests) * Heads(a, Cfg::ROWS).cut;
-    const bool by_head = cuts && cut_heads <= grid;
-    const int64_t bytes = cuts ? grid * (static_cast<int64_t>(sizeof(Record)) + piece_bytes<Cfg>()) : 0;
+    const Heads heads(a, Cfg::ROWS);
+    const int64_t cut_heads = static_cast<int64_t>(a.requests) * heads.cut;
+    Places places = {};
+    places.side = heads.cut % Cfg::WARPS == 0 ? Cfg::WARPS : heads.cut % 2 == 0 ? 2 : 1;
+    places.by_head = cuts && cut_heads <= static_cast<int64_t>(grid) * places.side;
+    places.floats = std::min(heads.group, static_cast<int>(Cfg::ROWS)) * Cfg::PITCH;
+    const int64_t list = places.by_head ? cut_heads : static_cast<int64_t>(grid) * places.side;
+    const int64_t bytes = cuts ? list * static_cast<int64_t>(sizeof(Record)) + 2ll * grid * places.side * places.floats * 4 : 0;
     if (need) {
         *need = bytes;
         return 0;
@@ -745,19 +828,24 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     if (bytes && (a.workspace_bytes < bytes || !a.workspace || !aligned16(a.workspace)))
         return refuse("paged_attend: a workspace of %lld bytes (16-byte aligned) is needed, not %lld", static_cast<long long>(bytes), static_cast<long long>(a.workspace_bytes));
     auto kernel = paged_attend_kernel<T, C, DIM, HT>;
-    static std::once_flag once[MAX_DEVICES];
+    static std::atomic<bool> sized[MAX_DEVICES];  // (threads that race here set the same value)
     int device = 0;
-    cudaGetDevice(&device);
-    std::call_once(once[device], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM); });
-    Record* records = cuts ? static_cast<Record*>(a.workspace) : nullptr;
-    float* pieces = cuts ? reinterpret_cast<float*>(records + grid) : nullptr;
-    if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), Cfg::THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), records, by_head, pieces))) return r;
+    if (cudaGetDevice(&device) != cudaSuccess) return refuse("paged_attend: no current device");
+    if (!sized[device].load(std::memory_order_acquire)) {
+        if (int r = launched("paged_attend's shared memory", cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM))) return r;
+        sized[device].store(true, std::memory_order_release);
+    }
+    if (cuts) {
+        places.records = static_cast<Record*>(a.workspace);
+        places.pieces = reinterpret_cast<float*>(places.records + list);
+    }
+    if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), Cfg::THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), places))) return r;
     if (!cuts) return 0;
     // about four CTAs an SM where records are few, each with as many warps for a row as its rows leave
-    const int list = by_head ? static_cast<int>(cut_heads) : grid, rows = std::min(a.heads / a.cache.kv_heads, static_cast<int>(Cfg::ROWS));
-    const int parts = std::max(1, std::min(rows, 4 * sms / list)), rows_each = (rows + parts - 1) / parts;
+    const int rows = std::min(heads.group, static_cast<int>(Cfg::ROWS));
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 4 * sms / list))), rows_each = (rows + parts - 1) / parts;
     const int split = rows_each >= 8 ? 1 : rows_each > 2 ? 2 : rows_each > 1 ? 4 : 8;
-    return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, HT>, dim3(list, parts), JOIN_WARPS * 32, 0, stream, a, records, pieces, split));
+    return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, HT>, dim3(static_cast<unsigned>(list), parts), JOIN_WARPS * 32, 0, stream, a, places, split));
 }
 
 template <class T, class C> int run_dim(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {

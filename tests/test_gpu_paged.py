@@ -362,6 +362,18 @@ def test_attend_long_many_and_ragged(paged, lengths, heads, kv_heads, dim, cache
     check_attend(paged, s)
 
 
+@pytest.mark.parametrize("lengths, heads, kv_heads, dim, dtype, cache", [
+    ([6000, 0, 7, 5000] * 20, 4, 4, 64, F16, F16), ([9000, 0, 7, 5000, 8000] * 12, 32, 8, 128, BF16, BF16), ([6000, 100, 5000] * 25, 8, 2, 128, F16, F16),
+    ([12000, 1, 9000] * 27, 24, 2, 128, BF16, BF16), ([9000, 0, 17, 12000] * 20, 16, 4, 64, BF16, E4M3), ([7000, 6000, 3] * 20, 4, 4, 128, F16, E4M3),
+    ([12000, 3, 9000] * 30, 8, 4, 256, BF16, E4M3), ([5000, 3, 900] * 25, 4, 4, 256, BF16, BF16), ([20000, 11, 20000] * 20, 40, 2, 64, BF16, E4M3)])
+@pytest.mark.parametrize("window", [0, 3000])
+def test_attend_heads_side_by_side(paged, lengths, heads, kv_heads, dim, dtype, cache, window):
+    """Batches that are large enough for a warp to have a head of its own."""
+    s = make_attend(lengths, heads, kv_heads, dim, dtype, cache, 16)
+    poison(s)
+    check_attend(paged, s, window=window)
+
+
 def test_attend_is_the_same_again(paged):
     """The split and the join have one order: two calls agree bit for bit."""
     s = make_attend([5000, 17, 900, 12000], 8, 2, 128, BF16, BF16, 16)
