@@ -36,9 +36,10 @@ namespace {
 using namespace emb::paged;
 namespace frag = emb::frag;
 
-// Where there are no more tiles than CTAs, a request's head of at most so many tiles is not cut: on a machine that is not
-// full a CTA takes about half a microsecond for a tile more, and the join two.
-constexpr int WHOLE_TILES = 4;
+// Where no request can have more than about so many keys, and there are no more tiles than CTAs, heads are not cut and
+// nothing is joined: four requests of 240 keys take 7.5 us so and 8.3 cut (128 dims, bf16), two of 900 keys 10.1 and 8.9 (64
+// dims, e4m3).
+constexpr int WHOLE_KEYS = 256;
 // Warps stand side by side where there are at least SIDE_SETS sets of heads for every 100 CTAs (a head is then spread over
 // few CTAs, and the join is short) and a CTA gets at least SIDE_TILES tiles (below, the latency of a head's keys one after
 // another counts, and they are better shared by the warps).
@@ -53,10 +54,10 @@ template <class T, class C, int DIM_, int HT_> struct Config {
     static constexpr bool CODES = sizeof(C) == 1;
     static constexpr bool BF16 = !CODES && std::is_same<T, __nv_bfloat16>::value;  // type of the products
     static constexpr int ROW_BYTES = DIM * static_cast<int>(sizeof(C));
-    static constexpr int KEYS = ROW_BYTES >= 256 || (ROW_BYTES == 128 && HT == 4) ? 16 : ROW_BYTES == 128 || HT == 4 ? 32 : 64;  // of a warp per step
+    static constexpr int KEYS = ROW_BYTES >= 256 ? 16 : ROW_BYTES == 128 ? 32 : 64;  // of a warp per step
     static constexpr int STEP_BYTES = 2 * KEYS * ROW_BYTES;                         // keys, then values
     static constexpr int WARPS = ROW_BYTES == 512 ? 2 : 4, THREADS = WARPS * 32;
-    static constexpr int CTAS = HT == 4 || (DIM * HT > 256 && ROW_BYTES < 512) ? 2 : 3;  // per SM
+    static constexpr int CTAS = 3;                                                  // per SM
     static constexpr int TILE = WARPS * KEYS;                                       // where the warps share a head
     static constexpr int TILE_SHIFT = (KEYS == 64 ? 6 : KEYS == 32 ? 5 : 4) + (WARPS == 4 ? 2 : 1);
     static_assert(TILE == 1 << TILE_SHIFT, "a power of two");
@@ -194,8 +195,8 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     constexpr int LOOKS = (KEYS + 31) / 32;  // keys that a lane looks up per step, at most
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long scan_slab[2][WARPS], share[2];
-    __shared__ long long first_before;  // tiles before the request that holds the share's first tile
-    __shared__ int first_request, holders;  // holders: CTAs from this one on that hold tiles of the head its share ends in
+    __shared__ uint32_t first_tile;
+    __shared__ int first_request, first_set, holders;  // the share's first tile; holders: CTAs from this one on that hold tiles of the head its share ends in
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, quad = lane & 3;
     follow_on();
     const Heads heads(a, Cfg::ROWS);
@@ -203,62 +204,72 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
 
     // ---- how the warps stand, and the CTA's share of the tiles
     const int side_shift = Cfg::TILE_SHIFT - (places.side >= 4 ? 2 : places.side >= 2 ? 1 : 0);
-    long long in_turn = 0, beside = 0;
-    for (int b = tid; b < a.requests; b += THREADS) {
-        const Span s = span_of(a, b);
-        in_turn += static_cast<long long>(tiles_of(s, Cfg::TILE_SHIFT)) * heads.cut;
-        beside += static_cast<long long>(tiles_of(s, side_shift)) * (heads.cut / places.side);
+    // tiles of the requests up to and with base + tid of this pass, in either way, and of all in the pass
+    const auto scan = [&](int base, const Span& s, long long& in_turn, long long& beside, long long (&sums)[2]) {
+        const bool real = base + tid < a.requests;
+        in_turn = real ? static_cast<long long>(tiles_of(s, Cfg::TILE_SHIFT)) * heads.cut : 0;
+        beside = real ? static_cast<long long>(tiles_of(s, side_shift)) * (heads.cut / places.side) : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, in_turn, d), y = __shfl_up_sync(0xffffffffu, beside, d);
+            if (lane >= d) in_turn += x, beside += y;
+        }
+        if (base) __syncthreads();  // the slab's last readers are done
+        if (lane == 31) scan_slab[0][warp] = in_turn, scan_slab[1][warp] = beside;
+        __syncthreads();
+        sums[0] = sums[1] = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) in_turn += scan_slab[0][w], beside += scan_slab[1][w];
+            sums[0] += scan_slab[0][w], sums[1] += scan_slab[1][w];
+        }
+    };
+    Span span = tid < a.requests ? span_of(a, tid) : Span{0, 0};
+    long long in_turn, beside, sums[2], totals[2];
+    scan(0, span, in_turn, beside, totals);
+    for (int base = THREADS; base < a.requests; base += THREADS) {
+        long long x, y;
+        scan(base, base + tid < a.requests ? span_of(a, base + tid) : Span{0, 0}, x, y, sums);
+        totals[0] += sums[0], totals[1] += sums[1];
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) in_turn += __shfl_xor_sync(0xffffffffu, in_turn, d), beside += __shfl_xor_sync(0xffffffffu, beside, d);
-    if (lane == 0) scan_slab[0][warp] = in_turn, scan_slab[1][warp] = beside;
-    __syncthreads();
-    in_turn = beside = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) in_turn += scan_slab[0][w], beside += scan_slab[1][w];
-    const bool stand = beside >= static_cast<long long>(SIDE_TILES) * gridDim.x && static_cast<long long>(a.requests) * (heads.cut / places.side) * 100 >= SIDE_SETS * static_cast<long long>(gridDim.x);
+    const bool stand = totals[1] >= static_cast<long long>(SIDE_TILES) * gridDim.x && static_cast<long long>(a.requests) * (heads.cut / places.side) * 100 >= SIDE_SETS * static_cast<long long>(gridDim.x);
     const int side = stand ? places.side : 1;
     const int sharing = WARPS / side;  // warps on one head
     const int shift = side > 1 ? side_shift : Cfg::TILE_SHIFT, sets = heads.cut / side;
     const int slot = warp / sharing, turn_of = warp % sharing;  // the warp's head in a set, and its turn among those on it
-    const long long all = side > 1 ? beside : in_turn;
+    const long long all = side > 1 ? totals[1] : totals[0];
     const long long n = min(static_cast<long long>(gridDim.x), all);
     if (static_cast<long long>(blockIdx.x) >= n) {
         if (tid < places.side && lists) places.records[blockIdx.x * places.side + tid].pieces = 0;
         return;
     }
-    const uint32_t whole = !places.pieces ? 0xffffffffu : all <= static_cast<long long>(gridDim.x) ? WHOLE_TILES : 0;  // no place for pieces: no cuts
-    if (tid < 2) share[tid] = all * (blockIdx.x + tid) / n;
-    if (tid == 0) holders = 0;
+    const bool whole = !places.pieces;  // no place for pieces: no cuts
+    const auto border = [&](uint32_t c) {  // all c / n; a 64-bit division takes longer than all else here
+        return all * (c + 1ll) < (1ll << 32) ? static_cast<long long>(static_cast<uint32_t>(all * c) / static_cast<uint32_t>(n)) : all * c / n;
+    };
+    const long long want0 = border(blockIdx.x), want1 = border(blockIdx.x + 1);
+    if (tid == 0) share[0] = want0, share[1] = want1, holders = 0;
     __syncthreads();
-    const long long want0 = share[0], want1 = share[1];
-    long long before_chunk = 0;
+    long long before_pass = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
-        const uint32_t tiles = base + tid < a.requests ? tiles_of(span_of(a, base + tid), shift) : 0u;
-        long long upto = static_cast<long long>(tiles) * sets;  // tiles up to and with request base + tid
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += x;
+        if (a.requests > THREADS) {  // (else the first scan's sums are at hand)
+            span = base + tid < a.requests ? span_of(a, base + tid) : Span{0, 0};
+            __syncthreads();
+            scan(base, span, in_turn, beside, sums);
         }
-        __syncthreads();  // the slab's last readers are done, and `share` is read
-        if (lane == 31) scan_slab[0][warp] = upto;
-        __syncthreads();
-        upto += before_chunk;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) upto += scan_slab[0][w];
-            before_chunk += scan_slab[0][w];
-        }
-        const long long from = upto - static_cast<long long>(tiles) * sets;
+        const uint32_t tiles = base + tid < a.requests ? tiles_of(span, shift) : 0u;
+        const long long upto = before_pass + (side > 1 ? beside : in_turn), from = upto - static_cast<long long>(tiles) * sets;
+        if (a.requests > THREADS) before_pass += side > 1 ? sums[1] : sums[0];
         // a border inside a head that is not to be cut moves to the head's first tile
         if (from <= want0 && want0 < upto) {
-            const long long x = tiles <= whole ? from + (want0 - from) / tiles * tiles : want0;
-            share[0] = x, first_request = base + tid, first_before = from;
+            const uint32_t ahead_of = static_cast<uint32_t>(want0 - from);  // (a request's tiles of all heads are fewer than 2^32)
+            const uint32_t set = ahead_of / tiles, t = whole ? 0 : ahead_of - set * tiles;
+            share[0] = from + static_cast<long long>(set) * tiles + t;
+            first_request = base + tid, first_set = set, first_tile = t;
         }
         if (from <= want1 && want1 < upto) {
-            const long long head_from = from + (want1 - from) / tiles * tiles;
-            if (tiles <= whole) share[1] = head_from;
+            const long long head_from = from + static_cast<long long>(static_cast<uint32_t>(want1 - from) / tiles) * tiles;
+            if (whole) share[1] = head_from;
             else if (head_from < want1) holders = static_cast<int>(((head_from + tiles) * n + all - 1) / all - blockIdx.x);
         }
     }
@@ -272,8 +283,8 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     ahead.b = first_request;
     ahead.span = span_of(a, ahead.b);
     ahead.tiles = tiles_of(ahead.span, shift);
-    ahead.set = static_cast<int>((x0 - first_before) / ahead.tiles);
-    ahead.t = static_cast<uint32_t>((x0 - first_before) % ahead.tiles);
+    ahead.set = first_set;
+    ahead.t = first_tile;
     Cursor now = ahead;
     const auto token_at = [&](const Cursor& c) { return (c.span.begin & ~15u) + (c.t << shift) + turn_of * KEYS; };  // the warp's first
 
@@ -313,7 +324,6 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
         const uint32_t kv = (ahead.set * side + slot) / heads.groups;
         // byte offsets of the rows (strides are below 2^32 elements), or the page id where there is no row
         long long k_at[LOOKS], v_at[LOOKS];
-        bool known = true;
 #pragma unroll
         for (int l = 0; l < LOOKS; ++l) {
             if (l && sixteens) break;
@@ -322,14 +332,16 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
             k_at[l] = one ? (id * k_stride[0] + static_cast<unsigned long long>(in_page[l]) * k_stride[1] + static_cast<unsigned long long>(kv) * k_stride[2]) * sizeof(C) : page[l] == -1 ? -1 : -2;
             v_at[l] = k_at[l];
             if (!same && one) v_at[l] = (id * v_stride[0] + static_cast<unsigned long long>(in_page[l]) * v_stride[1] + static_cast<unsigned long long>(kv) * v_stride[2]) * sizeof(C);
-            known = known && one;
         }
         const uint32_t to = ring + stage * Cfg::STEP_BYTES;
         const uint32_t token0 = token_at(ahead);
-        if (sixteens && __all_sync(0xffffffffu, known) && token0 >= ahead.span.begin && token0 + KEYS <= ahead.span.end) {
+        uint32_t rest = (1u << (KEYS / 16)) - 1;  // sixteens that are not copied whole
+        if (sixteens) {
 #pragma unroll
             for (int s = 0; s < KEYS / 16; ++s) {
                 const long long k_first = __shfl_sync(0xffffffffu, k_at[0], s), v_first = same ? k_first : __shfl_sync(0xffffffffu, v_at[0], s);
+                if (k_first < 0 || token0 + s * 16 < ahead.span.begin || token0 + s * 16 + 16 > ahead.span.end) continue;
+                rest &= ~(1u << s);
                 const char* k_row = k_from + k_first + (lane / CHUNKS) * k_step;
                 const char* v_row = v_from + v_first + (lane / CHUNKS) * v_step;
 #pragma unroll
@@ -340,11 +352,12 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                     k_row += k_step * PER_PASS, v_row += v_step * PER_PASS;
                 }
             }
-            return;
         }
+        if (!rest) return;
         // row by row: the ends of a span, pages that are not there, pages of other sizes
-#pragma unroll 2
+#pragma unroll 1
         for (int p = 0; p < KEYS / PER_PASS; ++p) {
+            if (!(rest >> (p * PER_PASS / 16) & 1)) continue;
             const int row = p * PER_PASS + lane / CHUNKS, source = sixteens ? row >> 4 : row & 31;
             const bool second = LOOKS > 1 && !sixteens && row >= 32;
             long long k_row = __shfl_sync(0xffffffffu, k_at[0], source), v_row = __shfl_sync(0xffffffffu, v_at[0], source);
@@ -812,7 +825,7 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     const int sms = sm_count();
     if (!sms) return refuse("paged_attend: the current device cannot be asked for its SMs");
     const int grid = grid_of<Cfg>(a, sms);
-    const bool cuts = grid == sms * Cfg::CTAS || longest_of(a) > WHOLE_TILES * Cfg::TILE;  // else no head is cut
+    const bool cuts = grid == sms * Cfg::CTAS || longest_of(a) > std::max(WHOLE_KEYS, static_cast<int>(Cfg::TILE));  // else no head is cut
     const Heads heads(a, Cfg::ROWS);
     const int64_t cut_heads = static_cast<int64_t>(a.requests) * heads.cut;
     Places places = {};
@@ -849,11 +862,13 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
 }
 
 template <class T, class C> int run_dim(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {
+    // a group of more query heads than a CTA's rows is cut into several, which read the same keys (at about the same time, so
+    // from L2): 32 query heads of 128 in one CTA need more registers than it has, and took 75 us where two of 16 take 50
     const int group = a.heads / a.cache.kv_heads;
     switch (a.cache.dim) {
-        case 64: return group <= 8 ? run<T, C, 64, 1>(a, stream, need) : group <= 16 ? run<T, C, 64, 2>(a, stream, need) : run<T, C, 64, 4>(a, stream, need);
-        case 128: return group <= 8 ? run<T, C, 128, 1>(a, stream, need) : group <= 16 ? run<T, C, 128, 2>(a, stream, need) : run<T, C, 128, 4>(a, stream, need);
-        default: return group <= 8 ? run<T, C, 256, 1>(a, stream, need) : run<T, C, 256, 2>(a, stream, need);
+        case 64: return group <= 8 ? run<T, C, 64, 1>(a, stream, need) : run<T, C, 64, 2>(a, stream, need);
+        case 128: return group <= 8 ? run<T, C, 128, 1>(a, stream, need) : run<T, C, 128, 2>(a, stream, need);
+        default: return run<T, C, 256, 1>(a, stream, need);
     }
 }
 
@@ -865,6 +880,7 @@ int attend(const emb_paged_attend_t* args, void* stream, int64_t* need) {
         return refuse("paged_attend: %d requests of %d heads over %d key heads: a multiple of the key heads", a.requests, a.heads, a.cache.kv_heads);
     if (a.table_width < 1 || static_cast<int64_t>(a.table_width) * a.cache.page_size >= (1ll << 31) - 1024 || a.table_stride < 0)
         return refuse("paged_attend: a table row of %d pages of %d tokens", a.table_width, a.cache.page_size);
+    if (static_cast<double>(a.table_width) * a.cache.page_size / 16 * a.heads >= 4.0e9) return refuse("paged_attend: a table row of %d pages of %d tokens for %d heads", a.table_width, a.cache.page_size, a.heads);
     if (a.window < 0) return refuse("paged_attend: a negative window");
     if (!(a.scale > -INFINITY && a.scale < INFINITY)) return refuse("paged_attend: the scale is not a finite number");
     if (need) *need = 0;
