@@ -5,6 +5,7 @@
 // were measured that way); here they are reads of the tensor's own fields. emmy_ptx/paged.py has the documented functions.
 
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -164,6 +165,13 @@ int device_of(const char* who, std::initializer_list<Arg> all) {
     return first.index();
 }
 
+// a tensor that wants its gradient would silently get none
+void no_graph(const char* who, std::initializer_list<Arg> all) {
+    if (!c10::GradMode::is_enabled()) return;
+    for (const Arg& x : all)
+        if (x.given() && x->requires_grad()) refuse("%s: %s requires a gradient, and this operator has none (call it under torch.no_grad())", who, x.name);
+}
+
 at::Tensor empty(c10::IntArrayRef shape, at::ScalarType type, int device) {
     return at::empty(shape, at::TensorOptions().dtype(type).device(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device))));
 }
@@ -233,6 +241,7 @@ PyObject* store(PyObject* const* o) {
     const Arg positions = tensor(who, "positions", o[6], true), rope = tensor(who, "rope", o[7], true);
     const Arg weights[2] = {tensor(who, "q_weight", o[8], true), tensor(who, "k_weight", o[9], true)};
     const Arg out = tensor(who, "out", o[14], true);
+    no_graph(who, {q, k, v, k_pages, v_pages, weights[0], weights[1]});
     emb_paged_store_t a;
     std::memset(&a, 0, sizeof a);
     a.dtype = q_type(who, q);
@@ -284,6 +293,7 @@ PyObject* attend(PyObject* const* o) {
     const Arg q = tensor(who, "q", o[0]), k_pages = tensor(who, "k_pages", o[1]), v_pages = tensor(who, "v_pages", o[2]);
     const Arg table = tensor(who, "table", o[3]), lengths = tensor(who, "lengths", o[4]);
     const Arg out = tensor(who, "out", o[9], true), lse = tensor(who, "lse", o[10], true);
+    no_graph(who, {q, k_pages, v_pages});
     emb_paged_attend_t a;
     std::memset(&a, 0, sizeof a);
     a.dtype = q_type(who, q);

@@ -735,75 +735,76 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
     }
 }
 
-// The pieces of the heads that were cut, a record and some rows of it for each CTA. A row's maximum and sum are joined as
-// in the kernel above. A row's pieces are dealt to `split` warps, whose parts are added in order: always the same order, so
-// results do not depend on timing. What it takes is the latency of three dependent loads, if a warp has few pieces.
+// The pieces of the heads that were cut. `split` warps (1, 2, 4 or 8) have a row of a record; its maximum and sum are joined as
+// in the kernel above. The warps' parts are added in order: always the same order, so results do not depend on timing. What it
+// takes is the latency of three dependent loads, if a warp has few pieces and all warps have a place at once. (A CTA for each
+// record took 12.8 us with a cold L2 where 1776 of them have two pieces of four rows.)
 constexpr int JOIN_WARPS = 8;
 
 template <class T, class C, int DIM, int HT>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const emb_paged_attend_t a, const Places places, int split) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const __grid_constant__ emb_paged_attend_t a, const Places places, const Divisor rows, uint32_t units, int split) {
     using Cfg = Config<T, C, DIM, HT>;
-    constexpr int PER_LANE = DIM / 32;
-    __shared__ float slab[JOIN_WARPS][Cfg::PITCH];
+    constexpr int PER_LANE = DIM / 32, BATCH = 4;  // dims of a lane; pieces loaded at a time
+    __shared__ __align__(16) float slab[JOIN_WARPS][DIM + 4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % split;
+    const uint32_t unit = (blockIdx.x * JOIN_WARPS + warp) / split, of = rows.over(unit);
+    const int r = unit - of * rows.d;
     follow_on();
-    const Record record = places.records[blockIdx.x];
-    if (record.pieces == 0) return;
     const Heads heads(a, Cfg::ROWS);
+    const Record record = unit < units ? places.records[of] : Record{};
     const int kv = record.head / heads.groups, row0 = (record.head % heads.groups) * Cfg::ROWS;
-    const int rows = min(Cfg::ROWS, heads.group - row0);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % split, at_once = JOIN_WARPS / split;
-    for (int base = blockIdx.y * at_once; base < rows; base += gridDim.y * at_once) {
-        const int r = min(base + warp / split, rows - 1);
+    const bool live = record.pieces > 0 && r < heads.group - row0;
+    float acc[PER_LANE] = {}, s = 0.f, best = LOWEST;
+    if (live) {
         // the first in its CTA's second place, the others in their CTAs' first
         const auto piece = [&](int i) -> const float* { return places.piece(record.cta + i, i == 0, record.slot) + r * Cfg::PITCH; };
-        float best = LOWEST;
         for (int k = lane; k < record.pieces; k += 32) best = fmaxf(best, piece(k)[DIM]);
-        float acc[PER_LANE] = {}, s = 0.f;
-        constexpr int BATCH = 4;
-        bool seen = false;
-        for (int k0 = part; k0 < record.pieces; k0 += BATCH * split) {
-            float x[BATCH][PER_LANE], top[BATCH], sum[BATCH];
+        for (int k0 = part; k0 < record.pieces || k0 == part; k0 += BATCH * split) {
+            float x[BATCH][PER_LANE];
+            float2 stat[BATCH];
 #pragma unroll
             for (int u = 0; u < BATCH; ++u) {
                 const float* const p = piece(min(k0 + u * split, record.pieces - 1));
-                top[u] = p[DIM], sum[u] = p[DIM + 1];
+                stat[u] = *reinterpret_cast<const float2*>(p + DIM);
 #pragma unroll
-                for (int e = 0; e < PER_LANE; ++e) x[u][e] = p[e * 32 + lane];
+                for (int e = 0; e < PER_LANE; e += 2) {
+                    const float2 y = *reinterpret_cast<const float2*>(p + lane * PER_LANE + e);
+                    x[u][e] = y.x, x[u][e + 1] = y.y;
+                }
             }
-            if (!seen) {  // (behind the first batch's loads)
+            if (k0 == part) {  // behind the first batch's loads
 #pragma unroll
                 for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-                seen = true;
             }
 #pragma unroll
             for (int u = 0; u < BATCH; ++u) {
                 if (k0 + u * split >= record.pieces) break;
-                const float f = exp2_(top[u] - best);
+                const float f = exp2_(stat[u].x - best);
 #pragma unroll
                 for (int e = 0; e < PER_LANE; ++e) acc[e] += f * x[u][e];
-                s += f * sum[u];
-            }
-        }
-        if (!seen) {
-#pragma unroll
-            for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-        }
-        __syncthreads();  // the last rows' parts are read
-#pragma unroll
-        for (int e = 0; e < PER_LANE; ++e) slab[warp][e * 32 + lane] = acc[e];
-        if (lane == 0) slab[warp][DIM] = s;
-        __syncthreads();
-        if (part == 0 && base + warp / split < rows) {
-            s = 0.f;
-            for (int w = 0; w < split; ++w) s += slab[warp + w][DIM];
-            for (int d = lane * 4; d < DIM; d += 128) {
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-                float none = 0.f;
-                for (int w = 0; w < split; ++w) add_part(sum, none, *reinterpret_cast<const float4*>(&slab[warp + w][d]), 1.f, 0.f);
-                put_out<Cfg, T>(a, record.request, static_cast<long long>(kv) * heads.group + row0 + r, d, sum, best, s);
+                s += f * stat[u].y;
             }
         }
     }
+    if (split > 1) {
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) slab[warp][lane * PER_LANE + e] = acc[e];
+        if (lane == 0) slab[warp][DIM] = s;
+        __syncthreads();
+        if (part) return;
+        for (int w = 1; w < split; ++w) {
+#pragma unroll
+            for (int e = 0; e < PER_LANE; ++e) acc[e] += slab[warp + w][lane * PER_LANE + e];
+            s += slab[warp + w][DIM];
+        }
+    }
+    if (!live) return;
+    const float inv = share_of<Cfg>(a, s);
+    const long long h = static_cast<long long>(kv) * heads.group + row0 + r;
+    T* const to = static_cast<T*>(a.out) + record.request * a.out_stride[0] + h * a.out_stride[1] + lane * PER_LANE;
+#pragma unroll
+    for (int e = 0; e < PER_LANE; e += 2) *reinterpret_cast<uint32_t*>(to + e) = frag::pack_f32<std::is_same<T, __nv_bfloat16>::value>(acc[e] * inv, acc[e + 1] * inv);
+    if (a.lse && lane == 0) a.lse[record.request * static_cast<long long>(a.heads) + h] = log_sum(best, s);
 }
 
 // no request's tiles cover more keys (one without a page among them where a length is beyond its table row, and up to 15
@@ -854,11 +855,12 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     }
     if (int r = launched("launch of paged_attend", launch(kernel, dim3(grid), Cfg::THREADS, Cfg::SMEM, stream, a, Divisor(a.cache.page_size), places))) return r;
     if (!cuts) return 0;
-    // about four CTAs an SM where records are few, each with as many warps for a row as its rows leave
+    // as many warps for a row as have a place at once
     const int rows = std::min(heads.group, static_cast<int>(Cfg::ROWS));
-    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 4 * sms / list))), rows_each = (rows + parts - 1) / parts;
-    const int split = rows_each >= 8 ? 1 : rows_each > 2 ? 2 : rows_each > 1 ? 4 : 8;
-    return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, HT>, dim3(static_cast<unsigned>(list), parts), JOIN_WARPS * 32, 0, stream, a, places, split));
+    const int64_t units = list * rows, at_once = 4ll * JOIN_WARPS * sms;
+    const int split = units * 8 <= at_once ? 8 : units * 4 <= at_once ? 4 : units * 2 <= at_once ? 2 : 1;
+    return launched("launch of paged_join", launch(paged_join_kernel<T, C, DIM, HT>, dim3(static_cast<unsigned>((units * split + JOIN_WARPS - 1) / JOIN_WARPS)), JOIN_WARPS * 32, 0, stream, a, places,
+                                                   Divisor(rows), static_cast<uint32_t>(units), split));
 }
 
 template <class T, class C> int run_dim(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {

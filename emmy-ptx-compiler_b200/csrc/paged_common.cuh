@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -76,15 +77,15 @@ constexpr int MAX_DEVICES = 64;
 
 // SMs of the current device; 0 where that cannot be had
 inline int sm_count() {
-    static int known[MAX_DEVICES];  // (threads that race here store the same number)
+    static std::atomic<int> known[MAX_DEVICES];  // (threads that race here store the same number)
     int device = -1;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= MAX_DEVICES) return 0;
-    if (!known[device]) {
-        int n = 0;
+    int n = known[device].load(std::memory_order_relaxed);
+    if (!n) {
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
-        known[device] = n;
+        known[device].store(n, std::memory_order_relaxed);
     }
-    return known[device];
+    return n;
 }
 
 // division by a number known to the host: floor(x / d) for x < 2^31

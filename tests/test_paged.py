@@ -105,6 +105,17 @@ def test_store_refuses(paged):
     refused(lambda: paged.store(q, k, v, k_pages, v_pages, slots, positions, out=rows(4)), "out is")
 
 
+def test_tensors_that_require_a_gradient_are_refused(paged):
+    k_pages, v_pages = pages()
+    q, k, v, slots, weight = rows(), rows(heads=2), rows(heads=2), i32(3), torch.zeros(64, dtype=torch.float16)
+    wanted = weight.clone().requires_grad_()
+    refused(lambda: paged.store(q, k, v, k_pages, v_pages, slots, slots, q_weight=wanted), "q_weight requires a gradient")
+    refused(lambda: paged.store(q, k.clone().requires_grad_(), v, k_pages, v_pages, slots, slots), "k requires a gradient")
+    refused(lambda: paged.attend(q.clone().requires_grad_(), k_pages, v_pages, i32(3, 2), slots), "q requires a gradient")
+    with torch.no_grad():  # then the next thing is refused
+        refused(lambda: paged.store(q, k, v, k_pages, v_pages, slots[:2], slots, q_weight=wanted), "slots is")
+
+
 def test_assign_refuses(paged):
     cached, fresh, table, free, head = i32(3), i32(3), i32(3, 4), i32(9), i32(1)
     refused(lambda: paged.assign(cached.long(), fresh, table, free, head, 16, 8), "cached is")
