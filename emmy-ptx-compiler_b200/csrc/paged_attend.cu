@@ -23,6 +23,13 @@
 // tiles [c T / n, (c + 1) T / n), whatever their requests. So a single long request and a ragged batch both spread evenly, and
 // a request's head is cut only where a CTA's share ends. Those pieces (maximum, sum, unscaled output; two per CTA at
 // most) go to the workspace, and paged_join_kernel adds them up in the order of the keys.
+//
+// Measured (a pass among others, join included; of the measured copy rate of 6.55 TB/s): 8 requests x 4096 keys x 32 key heads
+// of 128, f16, 537 MB: 88 us, 0.93 (the kernel alone 83 us, 0.99); 64 ragged requests up to 8192 keys, 32 query heads on 8 key
+// heads, bf16, 1070 MB: 169 us, 0.97; one request of 131072 keys, 537 MB: 90 us, 0.91; 128 requests of up to 2000 keys, 64
+// query heads on 8 key heads of 64, e4m3, 224 MB: 55 us, 0.62 (the decode of the codes: 45 % of the issue slots, with three
+// warps a scheduler to fill them; rows of 64 bytes come at 5 to 6.3 TB/s whatever reads them). Small calls are bound by latency:
+// 5.9 us for one request of 113 keys, 8 where pieces are joined.
 
 #include "paged_common.cuh"
 
@@ -47,7 +54,7 @@ constexpr int SIDE_SETS = 12, SIDE_TILES = 8;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 constexpr float LOWEST = -3.402823466e38f;  // seed of a maximum: finite, so that a masked score (-inf) against it weighs 0
-constexpr float SLACK = 8.f;
+constexpr float SLACK = 8.f;  // log2 of how far a score may pass the maximum that weights refer to
 
 template <class T, class C, int DIM_, int HT_> struct Config {
     static constexpr int DIM = DIM_, HT = HT_, ROWS = 8 * HT;  // query heads of a CTA, in tiles of eight
@@ -56,6 +63,9 @@ template <class T, class C, int DIM_, int HT_> struct Config {
     static constexpr int ROW_BYTES = DIM * static_cast<int>(sizeof(C));
     static constexpr int KEYS = ROW_BYTES >= 256 ? 16 : ROW_BYTES == 128 ? 32 : 64;  // of a warp per step
     static constexpr int STEP_BYTES = 2 * KEYS * ROW_BYTES;                         // keys, then values
+    // three CTAs with two steps of 8 KB a warp were faster than two with three: 86 against 98 us (64 requests up to 4000 keys,
+    // 8 key heads of 128, bf16), and than four or five with steps of half the keys (53 against 66 us, e4m3). Two steps in flight
+    // before the first wait instead of one were 2 to 3 % slower
     static constexpr int WARPS = ROW_BYTES == 512 ? 2 : 4, THREADS = WARPS * 32;
     static constexpr int CTAS = 3;                                                  // per SM
     static constexpr int TILE = WARPS * KEYS;                                       // where the warps share a head

@@ -10,8 +10,10 @@
 //   a' = r (a [w_a c] - b [w_b s]),  b' = r (b [w_b c] + a [w_a s]),  r = 1 / sqrt(mean + eps)
 // and the brackets are a token's and not a row's: a group of LANES lanes takes up to MOST_HEADS heads of one token, the
 // next AHEAD of them loaded while AHEAD are at work, and has the brackets, the slot and the addresses ready for all of them. A group has heads of one
-// kind only (q, k or v). (With the elements in order, the partners fetched by shuffles and heads of all kinds in a group the
-// arithmetic took longer than HBM: 130 us against 64 for 16384 tokens of 32 + 8 + 8 heads of 128, bf16.)
+// kind only (q, k or v). Measured on 16384 tokens of 32 + 8 + 8 heads of 128, bf16, 407 MB: 79 us = 5.15 TB/s, 0.79 of the
+// measured copy rate (with the elements in order, the partners fetched by shuffles and heads of all kinds in a group: 130 us;
+// 16-byte pieces of half as many lanes: 101; packed f32x2 arithmetic: no change, so it is not the arithmetic that bounds it
+// now but reads and 256-byte row writes mixed in HBM). Small steps are bound by the launch: 4.1 us a call for 8 to 256 tokens.
 
 #include <algorithm>
 
@@ -21,6 +23,7 @@ namespace {
 
 using namespace emb::paged;
 
+// 2, 8 and 8 CTAs an SM were the best of AHEAD 1, 2, 4, 8, MOST_HEADS 2 to 24 and 5 to 8 CTAs (79 us; the others 80 to 103)
 constexpr int THREADS = 128, AHEAD = 2, MOST_HEADS = 8;
 
 // how a launch's groups fall on a token: chunks of `heads` heads of q, of k and of v behind one another
