@@ -320,7 +320,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
             in_page[l] = token - index * page_size.d;
             page[l] = -1;
             if (token < ahead.span.end && (sixteens || token >= ahead.span.begin)) {
-                const uint32_t id = index < static_cast<uint32_t>(a.table_width) ? __ldg(a.table + ahead.b * a.table_stride + index) : -2;
+                const uint32_t id = index < static_cast<uint32_t>(a.table_width) ? a.table[ahead.b * a.table_stride + index] : -2;
                 page[l] = min(id, 0xfffffffeu);  // (an entry of -1 is a page that is not there, too)
             }
         }

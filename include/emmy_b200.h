@@ -263,7 +263,7 @@ int emb_paged_assign(const emb_paged_assign_t* args, void* stream);
  * they are) into slot slots[i] of the cache in the cache's type (e4m3: times
  * 1 / scale, nearest even, saturating). A slot outside the cache (negative among
  * them) stores nothing; its q_out is written. A position outside the table gives
- * NaN in the rotated dims. Two rows with the same slot: either's values. q_out may
+ * NaN in the rotated dims. Two rows with the same slot leave elements of either. q_out may
  * be q. A cache of 16-bit type has q's type. */
 typedef struct {
     const void* q; /* [tokens, heads, dim], q_stride = row, head */
