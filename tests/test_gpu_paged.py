@@ -232,6 +232,21 @@ def test_store_without_norm_and_in_place(paged):
     check_store(paged, 50, 4, 2, 128, 128, BF16, BF16, in_place=True)
 
 
+def test_store_takes_queries_out_of_a_wider_buffer_and_puts_them_into_one(paged):
+    gen = generator(9)
+    wide = normal((40, 20, 128), F16, gen)
+    q, k, v = wide[:, 2:10], wide[:, 11:13], wide[:, 17:19]
+    k_pages, v_pages = make_pages("pairs", 4, 16, 2, 128, F16, gen)
+    out = torch.full((40, 11, 128), 3.0, dtype=F16, device="cuda")
+    slots = torch.arange(40, device="cuda", dtype=torch.int32)
+    weight = normal((128,), F16, gen)
+    got = paged.store(q, k, v, k_pages, v_pages, slots, slots, q_weight=weight, out=out[:, 1:9])
+    assert got.data_ptr() == out[:, 1:9].data_ptr() and bool((out[:, 0] == 3).all()) and bool((out[:, 9:] == 3).all())
+    check_rows(got, *store_exact(q, weight, None, slots, False, 1e-6), F16)
+    at = slots.long()
+    assert torch.equal(k_pages[at // 16, at % 16], k) and torch.equal(v_pages[at // 16, at % 16], v)
+
+
 def test_store_extremes(paged):
     """A position outside the table shows as NaN in the rotated dims only; infinities saturate; no rows is no launch."""
     gen = generator(3)
@@ -372,6 +387,16 @@ def test_attend_heads_side_by_side(paged, lengths, heads, kv_heads, dim, dtype, 
     s = make_attend(lengths, heads, kv_heads, dim, dtype, cache, 16)
     poison(s)
     check_attend(paged, s, window=window)
+
+
+@pytest.mark.parametrize("size", [24, 7, 64])
+@pytest.mark.parametrize("layout", ["token", "head"])
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_attend_many_requests_side_by_side(paged, size, layout, cache):
+    """More requests than a CTA has threads, pages of other sizes, head-major pages."""
+    s = make_attend([2500, 300, 4000, 0] * 50, 8, 4, 64, BF16, cache, size, layout)
+    poison(s)
+    check_attend(paged, s)
 
 
 def test_attend_is_the_same_again(paged):
@@ -552,6 +577,35 @@ def test_two_captured_steps_run_at_once(paged):
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_calls_on_two_streams_at_once(paged):
+    cases = [make_attend([9000, 7, 900, 3000], 8, 2, 128, BF16, BF16, 16, seed=s) for s in (1, 2, 3, 4)]
+    want = [paged.attend(**c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(paged.attend(**c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_a_graph_of_several_layers_shares_its_memory(paged):
+    """Layers of one captured step: a later call's workspace may be an earlier one's, freed within the capture."""
+    cases = [make_attend([5000, 33, 1200], 8, 2, 64, F16, F16, 16, seed=s) for s in range(5)]
+    want = [paged.attend(**c) for c in cases]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = [paged.attend(**c) for c in cases]
+    for _ in range(5):
+        for x in got:
+            x.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, w) for x, w in zip(got, want))
 
 
 def test_a_captured_step_follows_its_lengths(paged):
