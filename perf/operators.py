@@ -8,7 +8,6 @@
 true. Both sides get what ``prepare`` made and return whole outputs: tables, caches and queries among them.
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -188,7 +187,6 @@ def prepare(case, seed):
 # ---------------------------------------------------------------- the framework's operators
 
 
-@functools.cache
 def _paged():
     root = str(Path.cwd() / "emmy-ptx-compiler_b200")
     if root not in sys.path:
