@@ -654,7 +654,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
 #pragma unroll
                         for (int half = 0; half < 2; ++half) most[m][e] = fmaxf(most[m][e], s[m][j][half * 2 + e]);
                     most[m][e] *= factor[m][e];
-                    passed |= most[m][e] > top[m][e] + SLACK;
+                    passed |= most[m][e] - top[m][e] > SLACK;  // (exact where it is near, whatever their size)
                 }
             if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
@@ -678,7 +678,9 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                 for (int j = 0; j < KT; ++j)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float u = exp2_(fmaf(s[m][j][half * 2], factor[m][0], -top[m][0])), v = exp2_(fmaf(s[m][j][half * 2 + 1], factor[m][1], -top[m][1]));
+                        // (the product is rounded as that of the maximum was: no weight passes 2^8, however large the scores)
+                        const float u = exp2_(__fsub_rn(__fmul_rn(s[m][j][half * 2], factor[m][0]), top[m][0]));
+                        const float v = exp2_(__fsub_rn(__fmul_rn(s[m][j][half * 2 + 1], factor[m][1]), top[m][1]));
                         total[m][0] += u, total[m][1] += v;
                         // the weights' one rounding: the product with the values takes 16-bit operands (f16 or bf16)
                         p[m][j][half] = transposed(frag::pack_f32<Cfg::BF16>(u, v));
