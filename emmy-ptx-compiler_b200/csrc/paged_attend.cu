@@ -16,8 +16,10 @@
 // The warps of a CTA either take the keys of one head in turn (a tile is WARPS * KEYS keys), and meet at the head's end, or,
 // where there is enough work and the number of heads allows, stand SIDE BY SIDE on neighbouring heads (a tile is KEYS keys of
 // each): then no warp waits for another, and a token's rows of several heads are read at about the same time.
-// The maximum that weights refer to moves only when a score passes it by more than 8 (a weight is at most 2^8, in f16 and f32
-// alike far from overflow): most steps then need neither the reduction over lanes nor the rescaling.
+// What weights refer to moves only when a score passes the maximum it came from by more than 8: most steps then need neither the
+// reduction over lanes nor the rescaling. For products of f16 it lies 7 below that maximum: a weight is at most 2^15, still below
+// f16's largest number, and the least that is not 0 is 2^-32 of the row's largest weight. (With the maximum itself it was 2^-25:
+// of 131072 keys that all have 2^-25.2 of the leading one's weight, 0.3 % of the result was lost.)
 //
 // The work is cut by TILES, all requests and heads (or sets of heads side by side) behind one another: CTA c of n takes
 // tiles [c T / n, (c + 1) T / n), whatever their requests. So a single long request and a ragged batch both spread evenly, and
@@ -54,12 +56,13 @@ constexpr int SIDE_SETS = 12, SIDE_TILES = 8;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 constexpr float LOWEST = -3.402823466e38f;  // seed of a maximum: finite, so that a masked score (-inf) against it weighs 0
-constexpr float SLACK = 8.f;  // log2 of how far a score may pass the maximum that weights refer to
+constexpr float SLACK = 8.f;  // log2 of how far a score may pass the maximum that what weights refer to came from
 
 template <class T, class C, int DIM_, int HT_> struct Config {
     static constexpr int DIM = DIM_, HT = HT_, ROWS = 8 * HT;  // query heads of a CTA, in tiles of eight
     static constexpr bool CODES = sizeof(C) == 1;
     static constexpr bool BF16 = !CODES && std::is_same<T, __nv_bfloat16>::value;  // type of the products
+    static constexpr float BELOW = BF16 ? 0.f : 7.f;  // log2: what weights refer to, below the maximum
     static constexpr int ROW_BYTES = DIM * static_cast<int>(sizeof(C));
     static constexpr int KEYS = ROW_BYTES >= 256 ? 16 : ROW_BYTES == 128 ? 32 : 64;  // of a warp per step
     static constexpr int STEP_BYTES = 2 * KEYS * ROW_BYTES;                         // keys, then values
@@ -654,7 +657,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
 #pragma unroll
                         for (int half = 0; half < 2; ++half) most[m][e] = fmaxf(most[m][e], s[m][j][half * 2 + e]);
                     most[m][e] *= factor[m][e];
-                    passed |= most[m][e] - top[m][e] > SLACK;  // (exact where it is near, whatever their size)
+                    passed |= most[m][e] - top[m][e] > SLACK + Cfg::BELOW;  // (exact where it is near, whatever their size)
                 }
             if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
@@ -664,7 +667,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                         float x = most[m][e];
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        const float raised = fmaxf(top[m][e], x), keep = exp2_(top[m][e] - raised);
+                        const float raised = fmaxf(top[m][e], x - Cfg::BELOW), keep = exp2_(top[m][e] - raised);
                         top[m][e] = raised;
                         total[m][e] *= keep;
 #pragma unroll
@@ -678,7 +681,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                 for (int j = 0; j < KT; ++j)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        // (the product is rounded as that of the maximum was: no weight passes 2^8, however large the scores)
+                        // (the product is rounded as that of the maximum was: no weight passes 2^15, however large the scores)
                         const float u = exp2_(__fsub_rn(__fmul_rn(s[m][j][half * 2], factor[m][0]), top[m][0]));
                         const float v = exp2_(__fsub_rn(__fmul_rn(s[m][j][half * 2 + 1], factor[m][1]), top[m][1]));
                         total[m][0] += u, total[m][1] += v;

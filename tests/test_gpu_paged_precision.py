@@ -1,4 +1,12 @@
-"""Attention over the pages where scores and weights reach the ends of their types' ranges."""
+"""Attention over the pages where scores and weights reach the ends of their types' ranges: what it loses to its 16-bit products.
+
+A weight is at most 2^-32 of the row's largest off below f16's range (what weights refer to lies 7 below the maximum, and half
+of f16's smallest step is 2^-25): sum_j |v_j| 2^-32 in all. The f32 sums of one long request are made of less than a thousand
+keys in each of the CTAs that it is spread over, and of one part of each of these, at most three on an SM: less than 2048 terms
+behind one another, 2^-13. The other terms are those of the general tests of the operators.
+"""
+
+import math
 
 import pytest
 import torch
@@ -31,6 +39,36 @@ def one_request(keys, values, page=16):
 
 
 @pytest.mark.parametrize("dtype, cache", [(F16, F16), (F16, E4M3), (BF16, E4M3), (BF16, BF16)])
+@pytest.mark.parametrize("n, bits", [(131072, 25.25), (131072, 24.6), (16385, 20.0), (70000, 23.5)])
+@pytest.mark.parametrize("heads", [4, 12])
+def test_a_long_flat_tail_beside_one_leading_key(paged, dtype, cache, n, bits, heads):
+    """The tail's weights are below f16's steps of the leading key's, and together part of the result."""
+    dim, lead = 64, n // 3
+    keys = torch.zeros(n, 1, dim, device="cuda")
+    keys[lead, 0, 0] = 16.0
+    values = torch.zeros(n, 1, dim, device="cuda")
+    values[:, 0, :32] = 1.0      # a constant stays one
+    values[lead, 0, 32:] = 1.0   # the leading key's share
+    values[:lead, 0, 48:] = -1.0
+    q = torch.zeros(1, heads, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    scale = bits * math.log(2) / 16
+    lse = torch.empty(1, heads, device="cuda")
+    got = paged.attend(q, *one_request(keys.to(cache), values.to(cache)), scale=scale, lse=lse)[0].double()
+    tail = (n - 1) * 2.0 ** -bits
+    total = 1.0 + tail
+    want = torch.empty(dim, dtype=torch.float64)
+    want[:32], want[32:48], want[48:] = 1.0, 1.0 / total, (1.0 - lead * 2.0 ** -bits) / total
+    u, w = torch.finfo(dtype).eps / 2, (2.0 ** -11 if cache is E4M3 else torch.finfo(cache).eps / 2)
+    spread = 16.0 * scale
+    # (of bf16 products a weight keeps its range: only f16 has the step of 2^-32)
+    tol = u + w + (0.0 if cache is BF16 else n * 2.0 ** -32) + 2.0 ** -13 + 2.0 ** -20 + spread * 2.0 ** -17
+    off = (got.cpu() - want).abs().max()
+    assert float(off) <= tol, (float(off), tol)
+    assert bool(((lse.double() - math.log(total) - spread).abs() <= spread * 2.0 ** -18 + 2.0 ** -20 + (spread + 1) * 2.0 ** -23 + 2.0 ** -13).all())
+
+
+@pytest.mark.parametrize("dtype, cache", [(F16, F16), (F16, E4M3), (BF16, E4M3), (BF16, BF16)])
 @pytest.mark.parametrize("scale", [3.0e5, 1.0e7, 3.0e9, 1.0e30, -1.0e7])
 def test_scores_as_large_as_they_come(paged, dtype, cache, scale):
     """Scores that lie apart by far more than their rounding: the largest one's key alone, and nothing overflows."""
@@ -44,3 +82,28 @@ def test_scores_as_large_as_they_come(paged, dtype, cache, scale):
     got = paged.attend(q, *one_request(keys.to(cache), values), scale=scale)
     best = int(order.argmax() if scale > 0 else order.argmin())
     assert torch.equal(got[0], values[best].to(dtype).expand(2, dim))
+
+
+@pytest.mark.parametrize("dtype, cache", [(F16, F16), (F16, E4M3), (BF16, BF16)])
+def test_a_flat_tail_that_one_warp_sums_up(paged, dtype, cache):
+    """As many requests as CTAs, all over the same pages, so that a warp has a head to itself: the tail's weights, 1.46 steps of
+    f16 below the leading key's 1, are not rounded to one step."""
+    n, dim, heads, bits = 262144, 64, 4, 23.45
+    requests = torch.cuda.get_device_properties(0).multi_processor_count * 3
+    keys = torch.zeros(n, 1, dim, device="cuda")
+    keys[5, 0, 0] = 16.0
+    values = torch.zeros(n, 1, dim, device="cuda")
+    values[5, 0, :32] = 1.0
+    values[6:, 0, 32:] = 1.0
+    q = torch.zeros(requests, heads, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    k_pages, v_pages, table, lengths = one_request(keys.to(cache), values.to(cache))
+    k_pages, v_pages = (p.expand(-1, -1, heads, -1) for p in (k_pages, v_pages))
+    got = paged.attend(q, k_pages, v_pages, table.expand(requests, -1), lengths.expand(requests).contiguous(), scale=bits * math.log(2) / 16).double()
+    tail = (n - 1) * 2.0 ** -bits
+    u, w = torch.finfo(dtype).eps / 2, (2.0 ** -11 if cache is E4M3 else torch.finfo(cache).eps / 2)
+    # a lane adds up an eighth of the weights (2^-24 each), a product sixteen keys (2^-23 each); weights of 2^-24 keep their bits in bf16
+    tol = u + w + n / 8 * 2.0 ** -24 + n / 16 * 2.0 ** -23 + 2.0 ** -20 + 16 * 2.0 ** -17
+    want = torch.tensor([1.0] * 32 + [(n - 6) * 2.0 ** -bits] * 32, dtype=torch.float64, device="cuda") / (1.0 + tail)
+    off = (got - want).abs().amax((0, 1))
+    assert float(off.max()) <= tol, (float(off[:32].max()), float(off[32:].max()), tol)
