@@ -20,6 +20,10 @@
 // reduction over lanes nor the rescaling. For products of f16 it lies 7 below that maximum: a weight is at most 2^15, still below
 // f16's largest number, and the least that is not 0 is 2^-32 of the row's largest weight. (With the maximum itself it was 2^-25:
 // of 131072 keys that all have 2^-25.2 of the leading one's weight, 0.3 % of the result was lost.)
+// A weight is two 16-bit numbers and so two products with the values (`split`). One alone is off by as much as the result's own
+// rounding: the mean error against 64 bits was 1.3 times that of a result rounded once. The second product costs under 1 %
+// where HBM is the bound (8 x 4096 keys 87.6 -> 88.1, 64 ragged requests 168.1 -> 168.8 us), 4 % over e4m3 codes with f16 queries
+// and 8 % with 16 query heads of 128 a key head (64 requests up to 4000 keys: 57.4 -> 62.1 us).
 //
 // The work is cut by TILES, all requests and heads (or sets of heads side by side) behind one another: CTA c of n takes
 // tiles [c T / n, (c + 1) T / n), whatever their requests. So a single long request and a ragged batch both spread evenly, and
@@ -63,6 +67,10 @@ template <class T, class C, int DIM_, int HT_> struct Config {
     static constexpr bool CODES = sizeof(C) == 1;
     static constexpr bool BF16 = !CODES && std::is_same<T, __nv_bfloat16>::value;  // type of the products
     static constexpr float BELOW = BF16 ? 0.f : 7.f;  // log2: what weights refer to, below the maximum
+    // whether a weight is held as two 16-bit numbers: where one would be off by as much as the result's own rounding is. (Over
+    // e4m3 codes the products are of f16, whose steps are an eighth of a bf16 result's; to split there too took 54 -> 57 us, 128
+    // requests of 2000 keys, 64-wide heads.)
+    static constexpr bool SPLIT = BF16 || std::is_same<T, __half>::value;
     static constexpr int ROW_BYTES = DIM * static_cast<int>(sizeof(C));
     static constexpr int KEYS = ROW_BYTES >= 256 ? 16 : ROW_BYTES == 128 ? 32 : 64;  // of a warp per step
     static constexpr int STEP_BYTES = 2 * KEYS * ROW_BYTES;                         // keys, then values
@@ -199,6 +207,22 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+
+// Two weights as one operand and what is left of them as another. The first parts are cut off a little below the weights, so
+// that what is left is never 0 beside a weight that is not: an infinite value stays infinite (0 * inf would be NaN).
+// Together they are off by at most 2^-20 of a weight (f16; 2^-25 where that is more) or 2^-14 (bf16).
+template <bool BF16> __device__ __forceinline__ void split(float u, float v, uint32_t& first, uint32_t& left) {
+    if (BF16) {
+        const uint32_t a = __float_as_uint(u * (1.f - 0x1p-7f)), b = __float_as_uint(v * (1.f - 0x1p-7f));
+        first = __byte_perm(a, b, 0x7632);
+        left = frag::pack_f32<true>(u - __uint_as_float(a & 0xffff0000u), v - __uint_as_float(b & 0xffff0000u));
+    } else {
+        const float a = fmaxf(fmaf(u, 1.f - 0x1p-10f, -0x1p-24f), 0.f), b = fmaxf(fmaf(v, 1.f - 0x1p-10f, -0x1p-24f), 0.f);
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(first) : "f"(b), "f"(a));
+        const float2 x = __half22float2(reinterpret_cast<const __half2&>(first));
+        left = frag::pack_f32<false>(u - x.x, v - x.y);
+    }
 }
 
 template <class T, class C, int DIM, int HT>
@@ -674,7 +698,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                         for (int d = 0; d < DT; ++d) o[m][d][e] *= keep, o[m][d][e + 2] *= keep;
                     }
             }
-            uint32_t p[HT][KT][2];
+            uint32_t p[HT][KT][2], left[HT][KT][2];  // the weights as operands
 #pragma unroll
             for (int m = 0; m < HT; ++m)
 #pragma unroll
@@ -685,8 +709,13 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                         const float u = exp2_(__fsub_rn(__fmul_rn(s[m][j][half * 2], factor[m][0]), top[m][0]));
                         const float v = exp2_(__fsub_rn(__fmul_rn(s[m][j][half * 2 + 1], factor[m][1]), top[m][1]));
                         total[m][0] += u, total[m][1] += v;
-                        // the weights' one rounding: the product with the values takes 16-bit operands (f16 or bf16)
-                        p[m][j][half] = transposed(frag::pack_f32<Cfg::BF16>(u, v));
+                        // the product with the values takes 16-bit operands (f16 or bf16)
+                        if (Cfg::SPLIT) {
+                            split<Cfg::BF16>(u, v, p[m][j][half], left[m][j][half]);
+                            p[m][j][half] = transposed(p[m][j][half]), left[m][j][half] = transposed(left[m][j][half]);
+                        } else {  // the weights' one rounding, to 2^-11
+                            p[m][j][half] = transposed(frag::pack_f32<Cfg::BF16>(u, v));
+                        }
                     }
 
             // ---- values
@@ -701,6 +730,8 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                         load4_trans(r, values + place<ROW_BYTES>(row, d * 2 + chunk));
 #pragma unroll
                         for (int m = 0; m < HT; ++m) frag::mma_f32<Cfg::BF16>(o[m][d], r, p[m][j]);
+#pragma unroll
+                        for (int m = 0; m < HT; ++m) frag::mma_f32<Cfg::BF16>(o[m][d], r, left[m][j]);
                     }
                 } else {
 #pragma unroll
@@ -715,6 +746,10 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                             widen4(__byte_perm(r[i + 2], 0, 0x3120), w[2], w[3]);
 #pragma unroll
                             for (int m = 0; m < HT; ++m) frag::mma_f32<false>(o[m][d + i], w, p[m][j]);
+                            if (Cfg::SPLIT) {
+#pragma unroll
+                                for (int m = 0; m < HT; ++m) frag::mma_f32<false>(o[m][d + i], w, left[m][j]);
+                            }
                         }
                     }
                 }

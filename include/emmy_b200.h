@@ -294,8 +294,9 @@ int emb_paged_store(const emb_paged_store_t* args, void* stream);
  * gives 0 (lse: -inf). What pages hold behind a request's length is not looked at
  * (NaN there does no harm). A table entry outside the cache, and a length beyond
  * the table row, give NaN in the request's outputs. Scores, their maximum and sum
- * and the output are held in f32; the weights are rounded to 16 bits (q's type;
- * f16 over an e4m3 cache) for the product with the values.
+ * and the output are held in f32. For the product with the values a weight is off
+ * by at most 2^-14 of it (bf16 caches), 2^-20 (f16 q) or 2^-11 (bf16 q over e4m3
+ * codes), and over f16 and e4m3 caches by 2^-32 of the row's largest weight.
  *   lse[b, h]  natural logarithm of the sum of exponentials, f32, contiguous; or NULL
  * A cache of 16-bit type has q's type. */
 typedef struct {

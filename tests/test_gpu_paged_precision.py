@@ -11,6 +11,8 @@ import math
 import pytest
 import torch
 
+from test_gpu_paged import make_attend, raw, rounding
+
 pytestmark = pytest.mark.gpu
 
 F16, BF16, E4M3 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
@@ -107,3 +109,42 @@ def test_a_flat_tail_that_one_warp_sums_up(paged, dtype, cache):
     want = torch.tensor([1.0] * 32 + [(n - 6) * 2.0 ** -bits] * 32, dtype=torch.float64, device="cuda") / (1.0 + tail)
     off = (got - want).abs().amax((0, 1))
     assert float(off.max()) <= tol, (float(off[:32].max()), float(off[32:].max()), tol)
+
+
+@pytest.mark.parametrize("dtype, cache", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(4, 2, 64), (8, 8, 128), (12, 1, 128), (24, 2, 64), (16, 1, 256)])
+def test_weights_have_more_bits_than_the_result(paged, dtype, cache, heads, kv_heads, dim):
+    """A weight is held to 2^-20 of it (f16) or 2^-14 (bf16), over e4m3 codes with a bf16 result to f16's 2^-11: the result is off by
+    little more than its own rounding, also where it is far smaller than the values it is made of."""
+    s = make_attend([1, 2, 3, 5, 9, 17, 40, 100], heads, kv_heads, dim, dtype, cache, 16, q_scale=0.25)
+    got = paged.attend(**s).double()
+    held = 2.0 ** -11 if (dtype, cache) == (BF16, E4M3) else 2.0 ** -20 if dtype is F16 else 2.0 ** -14
+    for b, n in enumerate(s["lengths"].tolist()):
+        j = torch.arange(n, device="cuda")
+        at = s["table"][b].long()[j // 16]
+        k, v = (raw(p)[at, j % 16].view(cache).double().repeat_interleave(heads // kv_heads, 1) * f
+                for p, f in ((s["k_pages"], s["k_scale"]), (s["v_pages"], s["v_scale"])))
+        x = s["q"][b].double() * dim ** -0.5
+        w = torch.einsum("hd,jhd->hj", x, k).softmax(1)
+        want, a = torch.einsum("hj,jhd->hd", w, v), torch.einsum("hj,jhd->hd", w, v.abs())
+        spread = torch.einsum("hd,jhd->hj", x.abs(), k.abs()).amax(1)[:, None]
+        tol = (held + n * 2.0 ** -24 + 2.0 ** -20 + spread * 2.0 ** -17) * a + rounding(want, dtype)
+        if cache is not BF16:
+            tol = tol + v.abs().sum(0) * 2.0 ** -32
+        off = (got[b] - want).abs()
+        assert bool((off <= tol).all()), (n, float((off / tol).max()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_an_infinite_value_stays_infinite(paged, dtype):
+    """Beside weights that a 16-bit number holds exactly (nothing is left of them) and others."""
+    s = make_attend([1, 4, 100], 4, 2, 64, dtype, dtype, 16)
+    for scale in (0.0, 0.125):
+        for b, at in ((0, 0), (1, 3), (2, 50)):
+            page, token = int(s["table"][b, at // 16]), at % 16
+            s["v_pages"][page, token, 1, 7] = math.inf
+            s["v_pages"][page, token, 0, 9] = -math.inf
+        got = paged.attend(**s, scale=scale)
+        assert (got[:, 2:, 7] == math.inf).all() and (got[:, :2, 9] == -math.inf).all()
+        got[:, 2:, 7] = got[:, :2, 9] = 0
+        assert got.isfinite().all()
