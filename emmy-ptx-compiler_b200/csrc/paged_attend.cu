@@ -465,8 +465,8 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
             float mine = scale;
             if (Cfg::CODES) {
                 // an e4m3 row's dims 4 quad .. 4 quad + 3 come in one word, so the query's dims are dealt the same way. The
-                // product is of f16: a bf16 query's row is first scaled by a power of two to 1 <= max < 2, so that it fits
-                // (what falls below 2^-24 of the row's maximum is rounded away, far below the query's own 2^-8 steps)
+                // product is of f16: a bf16 query's row is first scaled by a power of two to 2^14 <= max < 2^15, the top of
+                // f16's range (its 8 bits are kept down to 2^-28 of the row's maximum, and a rounding below is 2^-39 of it)
                 float most = 0.f;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__((Config<T, C, DIM, HT>::THREADS), (Config<T, C
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
                 int power = ((__float_as_int(most) >> 23) & 255) - 127;
-                power = std::is_same<T, __half>::value ? 0 : max(-100, min(power, 120));
+                power = std::is_same<T, __half>::value ? 0 : max(-100, min(power, 127)) - 14;
                 const float down = __int_as_float((127 - power) << 23);
                 mine = fmaxf(scale * __int_as_float((127 + power) << 23), 1.2e-38f);
 #pragma unroll

@@ -296,7 +296,8 @@ int emb_paged_store(const emb_paged_store_t* args, void* stream);
  * the table row, give NaN in the request's outputs. Scores, their maximum and sum
  * and the output are held in f32. For the product with the values a weight is off
  * by at most 2^-14 of it (bf16 caches), 2^-20 (f16 q) or 2^-11 (bf16 q over e4m3
- * codes), and over f16 and e4m3 caches by 2^-32 of the row's largest weight.
+ * codes), and over f16 and e4m3 caches by 2^-32 of the row's largest weight. Over
+ * e4m3 codes an element of a bf16 q is off by up to 2^-39 of its row's largest.
  *   lse[b, h]  natural logarithm of the sum of exponentials, f32, contiguous; or NULL
  * A cache of 16-bit type has q's type. */
 typedef struct {

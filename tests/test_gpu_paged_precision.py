@@ -148,3 +148,23 @@ def test_an_infinite_value_stays_infinite(paged, dtype):
         assert (got[:, 2:, 7] == math.inf).all() and (got[:, :2, 9] == -math.inf).all()
         got[:, 2:, 7] = got[:, :2, 9] = 0
         assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("largest", [2.0 ** 15, 2.0 ** 126, 2.0 ** -90])
+@pytest.mark.parametrize("ratio", [2.0 ** -12, 2.0 ** -20, 2.0 ** -27])
+@pytest.mark.parametrize("heads, dim", [(2, 64), (2, 128), (12, 128), (3, 256)])
+def test_small_elements_beside_a_large_one_in_a_query(paged, largest, ratio, heads, dim):
+    """The large element meets keys of 0, so the small ones make the scores: none of their bits is lost over e4m3 codes."""
+    n, gen = 40, torch.Generator("cuda").manual_seed(dim)
+    k, v = (torch.randn(n, 1, dim, device="cuda", generator=gen).to(E4M3) for _ in range(2))
+    k = k.float()
+    k[:, 0, 3] = 0
+    q = (torch.randn(1, heads, dim, device="cuda", generator=gen).clamp(-4, 4) * (largest * ratio / 4)).bfloat16()
+    q[:, :, 3] = largest
+    scale = 4 / (largest * ratio) * dim ** -0.5
+    got = paged.attend(q, *one_request(k.to(E4M3), v), scale=scale)[0].double()
+    x, k, v = q[0].double() * scale, k[:, 0].double(), v[:, 0].double()
+    w = (x @ k.T).softmax(1)
+    tol = (2.0 ** -11 + n * 2.0 ** -24 + 2.0 ** -20 + (x.abs() @ k.abs().T).amax(1)[:, None] * 2.0 ** -17) * (w @ v.abs()) + v.abs().sum(0) * 2.0 ** -32
+    off = (got - w @ v).abs() - rounding(w @ v, BF16) - tol
+    assert float(off.max()) <= 0, float(off.max())
