@@ -165,7 +165,7 @@ int device_of(const char* who, std::initializer_list<Arg> all) {
     return first.index();
 }
 
-// a tensor that wants its gradient would silently get none
+// a tensor that wants its gradient would silently get none (and one that is written would lose what it had)
 void no_graph(const char* who, std::initializer_list<Arg> all) {
     if (!c10::GradMode::is_enabled()) return;
     for (const Arg& x : all)
@@ -241,7 +241,7 @@ PyObject* store(PyObject* const* o) {
     const Arg positions = tensor(who, "positions", o[6], true), rope = tensor(who, "rope", o[7], true);
     const Arg weights[2] = {tensor(who, "q_weight", o[8], true), tensor(who, "k_weight", o[9], true)};
     const Arg out = tensor(who, "out", o[14], true);
-    no_graph(who, {q, k, v, k_pages, v_pages, weights[0], weights[1]});
+    no_graph(who, {q, k, v, k_pages, v_pages, rope, weights[0], weights[1], out});
     emb_paged_store_t a;
     std::memset(&a, 0, sizeof a);
     a.dtype = q_type(who, q);
@@ -293,7 +293,7 @@ PyObject* attend(PyObject* const* o) {
     const Arg q = tensor(who, "q", o[0]), k_pages = tensor(who, "k_pages", o[1]), v_pages = tensor(who, "v_pages", o[2]);
     const Arg table = tensor(who, "table", o[3]), lengths = tensor(who, "lengths", o[4]);
     const Arg out = tensor(who, "out", o[9], true), lse = tensor(who, "lse", o[10], true);
-    no_graph(who, {q, k_pages, v_pages});
+    no_graph(who, {q, k_pages, v_pages, out, lse});
     emb_paged_attend_t a;
     std::memset(&a, 0, sizeof a);
     a.dtype = q_type(who, q);
