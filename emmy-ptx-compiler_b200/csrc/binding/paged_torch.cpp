@@ -5,6 +5,7 @@
 // were measured that way); here they are reads of the tensor's own fields. emmy_ptx/paged.py has the documented functions.
 
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -165,11 +166,15 @@ int device_of(const char* who, std::initializer_list<Arg> all) {
     return first.index();
 }
 
-// a tensor that wants its gradient would silently get none (and one that is written would lose what it had)
+// a tensor that wants its gradient would silently get none (and one that is written would lose what it had); so would the
+// tangent of forward differentiation, which torch.no_grad() does not end
 void no_graph(const char* who, std::initializer_list<Arg> all) {
-    if (!c10::GradMode::is_enabled()) return;
-    for (const Arg& x : all)
-        if (x.given() && x->requires_grad()) refuse("%s: %s requires a gradient, and this operator has none (call it under torch.no_grad())", who, x.name);
+    const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const Arg& x : all) {
+        if (!x.given()) continue;
+        if (backward && x->requires_grad()) refuse("%s: %s requires a gradient, and this operator has none (call it under torch.no_grad())", who, x.name);
+        if (forward && x->_fw_grad(0).defined()) refuse("%s: %s has a tangent, and this operator has none", who, x.name);
+    }
 }
 
 at::Tensor empty(c10::IntArrayRef shape, at::ScalarType type, int device) {

@@ -7,7 +7,7 @@ each layer ``store`` (norm and rotation of the new queries and keys; keys and va
 
 Calls run on the current stream of the tensors' device, which need not be the current one, read nothing back and may be
 captured into a CUDA graph. Arguments that the host can judge are refused with ``driver.EmbError`` (code -2). There is no
-gradient: a tensor that requires one is refused where gradients are on.
+gradient: a tensor that requires one is refused where gradients are on, and so is one with a tangent (forward mode).
 """
 
 from __future__ import annotations

@@ -46,3 +46,17 @@ def test_each_tensor_that_requires_a_gradient_is_refused(paged, name, argument):
     refused(paged, name, arguments, f"{argument} requires a gradient")
     with torch.no_grad():  # then it is the device that is refused
         refused(paged, name, arguments, "GPU only")
+
+
+@pytest.mark.parametrize("name, argument", FLOATS)
+def test_each_tensor_with_a_tangent_is_refused(paged, name, argument):
+    from torch.autograd import forward_ad
+    arguments = store_arguments() if name == "store" else attend_arguments()
+    plain = arguments[argument]
+    with forward_ad.dual_level():
+        arguments[argument] = forward_ad.make_dual(plain, torch.ones_like(plain))
+        refused(paged, name, arguments, f"{argument} has a tangent")
+        with torch.no_grad():
+            refused(paged, name, arguments, f"{argument} has a tangent")
+        arguments[argument] = plain  # then it is the device that is refused
+        refused(paged, name, arguments, "GPU only")
