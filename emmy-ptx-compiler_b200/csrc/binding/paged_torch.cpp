@@ -177,6 +177,13 @@ void no_graph(const char* who, std::initializer_list<Arg> all) {
     }
 }
 
+// what an operator wrote into, for autograd: a graph that saved one of these tensors finds that it changed. (Tensors made in
+// inference mode have no count.)
+void wrote(std::initializer_list<Arg> all) {
+    for (const Arg& x : all)
+        if (x.given() && !x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor empty(c10::IntArrayRef shape, at::ScalarType type, int device) {
     return at::empty(shape, at::TensorOptions().dtype(type).device(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device))));
 }
@@ -230,7 +237,9 @@ PyObject* assign(PyObject* const* o) {
     a.slots = to[0], a.positions = to[1], a.starts = to[2], a.lengths = to[3], a.free_head_out = to[4], a.report = to[5];
     const c10::cuda::OptionalCUDAGuard guard(static_cast<c10::DeviceIndex>(device));
     check(emb_paged_assign(&a, c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream()));
+    wrote({table});
     if (given != Py_None) {
+        for (int i = 0; i < 6; ++i) wrote({tensor(who, names[i], PyTuple_GET_ITEM(given, i))});
         Py_INCREF(given);
         return given;
     }
@@ -288,6 +297,7 @@ PyObject* store(PyObject* const* o) {
     a.q_out = out.given() ? out->data_ptr() : made.data_ptr();
     const c10::cuda::OptionalCUDAGuard guard(static_cast<c10::DeviceIndex>(device));
     check(emb_paged_store(&a, c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream()));
+    wrote({k_pages, v_pages, out});
     if (!out.given()) return THPVariable_Wrap(std::move(made));
     Py_INCREF(o[14]);
     return o[14];
@@ -337,6 +347,7 @@ PyObject* attend(PyObject* const* o) {
         a.workspace = workspace.get();
     }
     check(emb_paged_attend(&a, c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream()));
+    wrote({out, lse});
     if (!out.given()) return THPVariable_Wrap(std::move(made));
     Py_INCREF(o[9]);
     return o[9];
