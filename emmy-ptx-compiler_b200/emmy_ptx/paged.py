@@ -70,7 +70,7 @@ def store(q, k, v, k_pages, v_pages, slots, positions, rope=None, q_weight=None,
     order of the first three dimensions. ``slots``, ``positions`` [tokens] int32; a slot of -1 stores nothing. ``rope``
     [positions, rot] f32: rot/2 cosines, then rot/2 sines; pairs (j, j + rot/2), or (2j, 2j + 1) where ``interleaved``.
     ``q_weight``, ``k_weight`` [dim]: y = x / sqrt(mean(x^2) + eps) * weight over each head; None: no norm. ``out`` may
-    be ``q``.
+    be ``q``; other memory that the call reads, or writes elsewhere, is refused as an output.
     """
     return (_native or _load()).store(q, k, v, k_pages, v_pages, slots, positions, rope, q_weight, k_weight, eps, interleaved, k_scale, v_scale, out)
 

@@ -264,7 +264,10 @@ int emb_paged_assign(const emb_paged_assign_t* args, void* stream);
  * 1 / scale, nearest even, saturating). A slot outside the cache (negative among
  * them) stores nothing; its q_out is written. A position outside the table gives
  * NaN in the rotated dims. Two rows with the same slot leave elements of either. q_out may
- * be q. A cache of 16-bit type has q's type. */
+ * be q, with its strides; else what is written (q_out, keys' pages, values' pages)
+ * may share no byte with anything read or written (views of one buffer whose rows lie
+ * between one another's are apart; memory strided in ways too odd to tell is refused).
+ * A cache of 16-bit type has q's type. */
 typedef struct {
     const void* q; /* [tokens, heads, dim], q_stride = row, head */
     const void* k; /* [tokens, kv_heads, dim] */

@@ -1,0 +1,124 @@
+"""Memory that an operator of the paged cache would write while it reads it, or write twice: refused by the host.
+
+The calls here carry addresses that no launch may ever see, so they run only where no GPU can: an accepted call ends at the
+question for the device's SMs.
+"""
+
+import ctypes
+import random
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from test_paged import ASSIGN, ATTEND, STORE, cache_fields
+
+ROOT = Path(__file__).resolve().parents[1]
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are not there")
+
+HARNESS = '''
+#include <cstdio>
+#include "paged_overlap.h"
+using namespace emb::paged;
+int main() {
+    long long at[2], run[2], n[2], c[2][3], s[2][3];
+    for (;;) {
+        for (int i = 0; i < 2; ++i) {
+            if (std::scanf("%lld %lld %lld", &at[i], &run[i], &n[i]) != 3) return 0;
+            for (int k = 0; k < n[i]; ++k) if (std::scanf("%lld %lld", &c[i][k], &s[i][k]) != 2) return 1;
+        }
+        Area a("a", reinterpret_cast<void*>(at[0]), run[0]), b("b", reinterpret_cast<void*>(at[1]), run[1]);
+        for (int k = 0; k < n[0]; ++k) a.by(c[0][k], s[0][k]);
+        for (int k = 0; k < n[1]; ++k) b.by(c[1][k], s[1][k]);
+        std::printf("%d%d", touch(a, b), touch(b, a));
+    }
+}
+'''
+
+
+def covered(at, run, dims):
+    starts = [at]
+    for c, s in dims:
+        starts = [x + i * s for x in starts for i in range(c)]
+    return {x + i for x in starts for i in range(run)}
+
+
+def test_areas_touch_where_their_bytes_do(tmp_path):
+    (tmp_path / "t.cpp").write_text(HARNESS)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-I", str(ROOT / "emmy-ptx-compiler_b200" / "csrc"), "-o", str(tmp_path / "t"), str(tmp_path / "t.cpp")], check=True)
+    rng = random.Random(5)
+    cases = []
+    for _ in range(4000):
+        shared = [rng.choice((0, 4, 8, 12, 16, 24, 40, 64, 100, 160)) for _ in range(3)]  # the strides of views of one buffer, or of two
+        one = []
+        for side in range(2):
+            dims = [(rng.choice((0, 1, 2, 3, 5)) if rng.random() < 0.1 else rng.randint(1, 5), s if rng.random() < 0.7 else rng.choice((4, 6, 20, 36, 80))) for s in shared[:rng.randint(0, 3)]]
+            one.append((rng.randint(1, 300) if side else 150, rng.choice((1, 2, 4, 8, 16)), dims))
+        cases.append(one)
+    text = "\n".join(" ".join(f"{at} {run} {len(dims)} " + " ".join(f"{c} {s}" for c, s in dims) for at, run, dims in one) for one in cases)
+    got = subprocess.run([str(tmp_path / "t")], input=text, capture_output=True, text=True, check=True).stdout
+    want = ["11" if covered(*a) & covered(*b) else "00" for a, b in cases]
+    assert [got[2 * i:2 * i + 2] for i in range(len(cases))] == want
+    assert 500 < want.count("11") < 3500
+
+
+class Call:
+    def __init__(self, name, struct_):
+        import __graft_entry__ as g
+        g.build_binding()
+        from emmy_ptx import driver
+        self.library = driver.library()
+        self.entry, self.struct = getattr(self.library, f"emb_paged_{name}"), struct_
+        self.entry.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+
+    def text(self, fields):
+        code = self.entry(self.struct.pack(*fields), None)
+        assert code != 0
+        return self.library.emb_last_error().decode()
+
+
+def flat(f, changes):
+    f.update(changes)
+    return [x for v in f.values() for x in (v if isinstance(v, list) else [v])]
+
+
+# ---- store: 20 tokens of 4 + 2 + 2 heads of 64, 16 bits; a projection's row has 8 heads, 1024 bytes; the pages 4 x 16 x 2 heads
+
+Q, K, V, KP, VP, OUT, SMALL = (x << 20 for x in range(1, 8))
+
+
+def store_fields(cache=(), **changes):
+    cache = dict(dict(k=KP, v=VP), **dict(cache))
+    return flat(dict(q=Q, k=K, v=V, out=OUT, slots=SMALL, positions=SMALL + 4096, rope=SMALL + 8192, qw=SMALL + 65536, kw=SMALL + 65792, cache=cache_fields(**cache), q0=256,
+                     q1=64, k0=128, k1=64, v0=128, v1=64, o0=256, o1=64, tokens=20, heads=4, dtype=1, rot=64, rope_rows=8, interleaved=0, eps=1e-6, r=0), changes)
+
+
+QKV = dict(q=Q, k=Q + 512, v=Q + 768, q0=512, k0=512, v0=512)
+PAIRS = dict(k=KP, v=KP + 4096, ks0=4096, vs0=4096)  # keys and values of a page behind one another
+
+STORE_APART = [
+    dict(), dict(out=Q), QKV, dict(QKV, out=Q, o0=512), dict(QKV, q=Q + 128, k=Q + 640, v=Q + 896, q0=768, k0=768, v0=768, o0=768, out=Q + 1152),
+    dict(out=Q + 20 * 512), dict(cache=PAIRS), dict(cache=dict(PAIRS, k=KP, v=KP + 128, ks0=4096, vs0=4096, ks1=256, vs1=256, ks2=128, vs2=128)),
+    dict(cache=dict(PAIRS, v=KP + 256, ks0=4096, vs0=4096, ks1=256, vs1=256)), dict(tokens=1, out=Q, q0=0, o0=0), dict(rot=0, rope=OUT, positions=OUT),
+    dict(qw=0, kw=0), dict(slots=SMALL, positions=SMALL), dict(q0=0, out=Q + 512), dict(k0=0, v0=0, k=Q, v=Q)]
+STORE_TOUCH = [
+    (dict(out=Q + 128), "q_out and q"), (dict(out=Q + 256, o0=512), "q_out and q"), (dict(out=Q, o0=512), "q_out and q"), (dict(q0=0, out=Q), "q_out and q"),
+    (dict(QKV, out=Q + 128, o0=512), "q_out and q"), (dict(QKV, out=Q + 512, o0=512), "q_out and k"), (dict(QKV, q=Q + 16384 * 4, out=Q + 384, o0=512), "q_out and k"),
+    (dict(QKV, q=Q + 128, k=Q + 640, v=Q + 896, q0=768, k0=768, v0=768, o0=768, out=Q + 1024), "q_out and v"),
+    (dict(k=OUT + 9728 + 384, k0=128), "q_out and k"), (dict(out=V - 16, o0=256), "q_out and v"), (dict(out=V + 20 * 256 - 16), "q_out and v"),
+    (dict(out=KP + 16368), "q_out and the keys' pages"), (dict(out=VP), "q_out and the values' pages"), (dict(cache=dict(v=KP)), "the keys' pages and the values' pages"),
+    (dict(cache=dict(v=KP + 2048)), "the keys' pages and the values' pages"), (dict(cache=dict(PAIRS, v=KP + 4096 - 128)), "the keys' pages and the values' pages"),
+    (dict(k=KP + 4096), "the keys' pages and k"), (dict(v=KP), "the keys' pages and v"), (dict(q=VP + 128), "the values' pages and q"), (dict(slots=OUT + 512), "q_out and slots"),
+    (dict(positions=KP + 64), "the keys' pages and positions"), (dict(rope=VP + 16), "the values' pages and rope"), (dict(qw=OUT), "q_out and q_weight"),
+    (dict(kw=KP + 16384 - 16), "the keys' pages and k_weight")]
+
+
+@pytest.mark.parametrize("changes", STORE_APART)
+def test_store_takes_memory_that_is_apart(changes):
+    assert "cannot be asked for its SMs" in Call("store", STORE).text(store_fields(**changes))
+
+
+@pytest.mark.parametrize("changes, match", STORE_TOUCH)
+def test_store_refuses_memory_that_it_writes_and_reads(changes, match):
+    assert Call("store", STORE).text(store_fields(**changes)) == f"paged_store: {match} share memory"
