@@ -871,6 +871,18 @@ template <class Cfg> int grid_of(const emb_paged_attend_t& a, int sms) {
     return most < all ? static_cast<int>(most) : all;
 }
 
+// (out may be q: a head's queries are in registers before its output is written, by the CTA that has the head to itself or by
+// the join.) `workspace`: its bytes, where the call has been found to need one
+int check_overlap(const emb_paged_attend_t& a, int64_t workspace) {
+    const Area written[3] = {rows_at("out", a.out, a.requests, a.heads, a.cache.dim, a.out_stride), Area("lse", a.lse, wide(a.requests) * a.heads * 4),
+                             Area("the workspace", workspace ? a.workspace : nullptr, workspace)};
+    const Area read[5] = {rows_at("q", a.q, a.requests, a.heads, a.cache.dim, a.q_stride), pages_at("the keys' pages", a.cache, a.cache.k, a.cache.k_stride),
+                          pages_at("the values' pages", a.cache, a.cache.v, a.cache.v_stride),
+                          Area("table", a.table, wide(a.table_width) * 4).by(a.requests, wide(a.table_stride) * 4), Area("lengths", a.lengths, wide(a.requests) * 4)};
+    const char* which[2];
+    return touches(written, read, &read[0], which) ? refuse("paged_attend: %s and %s share memory", which[0], which[1]) : 0;
+}
+
 template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {
     using Cfg = Config<T, C, DIM, HT>;
     const int sms = sm_count();
@@ -891,6 +903,7 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     }
     if (bytes && (a.workspace_bytes < bytes || !a.workspace || !aligned16(a.workspace)))
         return refuse("paged_attend: a workspace of %lld bytes (16-byte aligned) is needed, not %lld", static_cast<long long>(bytes), static_cast<long long>(a.workspace_bytes));
+    if (int r = bytes ? check_overlap(a, bytes) : 0) return r;
     auto kernel = paged_attend_kernel<T, C, DIM, HT>;
     static std::atomic<bool> sized[MAX_DEVICES];  // (threads that race here set the same value)
     int device = 0;
@@ -944,6 +957,7 @@ int attend(const emb_paged_attend_t* args, void* stream, int64_t* need) {
             if (!stride_fits(s[0], 2) || !stride_fits(s[1], 2)) return refuse("paged_attend: a stride of q or out is not a multiple of 16 bytes below 2^32 elements");
         const int64_t rows[2] = {a.requests, a.heads};
         if (!rows_apart(rows, a.out_stride, a.cache.dim)) return refuse("paged_attend: rows of out overlap");
+        if (int r = check_overlap(a, 0)) return r;
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a.dtype == EMB_F16) return a.cache.dtype == EMB_U8 ? run_dim<__half, E4m3>(a, s, need) : run_dim<__half, __half>(a, s, need);

@@ -13,6 +13,7 @@
 #include <cstdio>
 
 #include "emmy_b200.h"
+#include "paged_overlap.h"
 
 int emb_fail_text(int code, const char* text);  // shim.cpp
 
@@ -71,6 +72,15 @@ inline int check_cache(const char* who, const emb_paged_cache_t& c, int q_dtype)
             return refuse("%s: a stride of the pages is not a multiple of 16 bytes below 2^32 elements", who);
     if (!(c.k_scale > 0.f) || !(c.v_scale > 0.f) || c.k_scale > 3.0e38f || c.v_scale > 3.0e38f) return refuse("%s: a cache scale is not a positive number", who);
     return 0;
+}
+
+// rows [n, heads, dim] of 16 bits, and the pages of a cache
+inline Area rows_at(const char* name, const void* p, int64_t n, int heads, int dim, const int64_t (&stride)[2]) {
+    return Area(name, p, dim * 2).by(heads, wide(stride[1]) * 2).by(n, wide(stride[0]) * 2);
+}
+inline Area pages_at(const char* name, const emb_paged_cache_t& c, const void* p, const int64_t (&stride)[3]) {
+    const int size = c.dtype == EMB_U8 ? 1 : 2;
+    return Area(name, p, c.dim * size).by(c.kv_heads, wide(stride[2]) * size).by(c.page_size, wide(stride[1]) * size).by(c.pages, wide(stride[0]) * size);
 }
 
 constexpr int MAX_DEVICES = 64;

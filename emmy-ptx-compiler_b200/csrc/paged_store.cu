@@ -18,7 +18,6 @@
 #include <algorithm>
 
 #include "paged_common.cuh"
-#include "paged_overlap.h"
 
 namespace {
 
@@ -193,15 +192,12 @@ extern "C" int emb_paged_store(const emb_paged_store_t* args, void* stream) {
     const int64_t rows[2] = {a.tokens, a.heads}, slots[3] = {a.cache.pages, a.cache.page_size, a.cache.kv_heads};
     if (!rows_apart(rows, a.out_stride, a.cache.dim)) return refuse("paged_store: rows of q_out overlap");
     if (!rows_apart(slots, a.cache.k_stride, a.cache.dim) || !rows_apart(slots, a.cache.v_stride, a.cache.dim)) return refuse("paged_store: slots of the cache overlap");
-    const auto rows_at = [&](const char* name, const void* p, const int64_t* stride, int heads) { return Area(name, p, a.cache.dim * 2).by(heads, stride[1] * 2).by(a.tokens, stride[0] * 2); };
-    const auto pages_at = [&](const char* name, const void* p, const int64_t* stride) {
-        const int size = a.cache.dtype == EMB_U8 ? 1 : 2;
-        return Area(name, p, a.cache.dim * size).by(a.cache.kv_heads, wide(stride[2]) * size).by(a.cache.page_size, wide(stride[1]) * size).by(a.cache.pages, wide(stride[0]) * size);
-    };
-    const Area written[3] = {rows_at("q_out", a.q_out, a.out_stride, a.heads), pages_at("the keys' pages", a.cache.k, a.cache.k_stride), pages_at("the values' pages", a.cache.v, a.cache.v_stride)};
-    const Area read[8] = {rows_at("q", a.q, a.q_stride, a.heads), rows_at("k", a.k, a.k_stride, a.cache.kv_heads), rows_at("v", a.v, a.v_stride, a.cache.kv_heads),
-                          Area("slots", a.slots, a.tokens * wide(4)), Area("positions", a.rot ? a.positions : nullptr, a.tokens * wide(4)),
-                          Area("rope", a.rot ? a.rope : nullptr, wide(a.rope_rows) * a.rot * 4), Area("q_weight", a.q_weight, a.cache.dim * 2), Area("k_weight", a.k_weight, a.cache.dim * 2)};
+    const int n = a.tokens, kv_heads = a.cache.kv_heads, dim = a.cache.dim;
+    const Area written[3] = {rows_at("q_out", a.q_out, n, a.heads, dim, a.out_stride), pages_at("the keys' pages", a.cache, a.cache.k, a.cache.k_stride),
+                             pages_at("the values' pages", a.cache, a.cache.v, a.cache.v_stride)};
+    const Area read[8] = {rows_at("q", a.q, n, a.heads, dim, a.q_stride), rows_at("k", a.k, n, kv_heads, dim, a.k_stride), rows_at("v", a.v, n, kv_heads, dim, a.v_stride),
+                          Area("slots", a.slots, n * wide(4)), Area("positions", a.rot ? a.positions : nullptr, n * wide(4)),
+                          Area("rope", a.rot ? a.rope : nullptr, wide(a.rope_rows) * a.rot * 4), Area("q_weight", a.q_weight, dim * 2), Area("k_weight", a.k_weight, dim * 2)};
     const char* which[2];
     if (touches(written, read, &read[0], which)) return refuse("paged_store: %s and %s share memory", which[0], which[1]);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

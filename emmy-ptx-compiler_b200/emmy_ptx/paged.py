@@ -83,6 +83,7 @@ def attend(q, k_pages, v_pages, table, lengths, scale: float | None = None, wind
     h // (heads // key heads). ``table`` [requests, width] and ``lengths`` [requests] int32: key j of request b is token
     j % page size of page table[b, j // page size], j < lengths[b], the new token's own among them; ``window``: only the
     last so many (0: all). ``scale``: 1 / sqrt(dim) where None. A request of length 0 gives 0. ``lse`` [requests, heads]
-    f32: written with the logarithm of the sum of exponentials.
+    f32: written with the logarithm of the sum of exponentials. ``out`` may be ``q``; other memory that the call reads is
+    refused as an output.
     """
     return (_native or _load()).attend(q, k_pages, v_pages, table, lengths, scale, window, k_scale, v_scale, out, lse)

@@ -302,7 +302,8 @@ int emb_paged_store(const emb_paged_store_t* args, void* stream);
  * codes), and over f16 and e4m3 caches by 2^-32 of the row's largest weight. Over
  * e4m3 codes an element of a bf16 q is off by up to 2^-39 of its row's largest.
  *   lse[b, h]  natural logarithm of the sum of exponentials, f32, contiguous; or NULL
- * A cache of 16-bit type has q's type. */
+ * out may be q, with its strides; else out, lse and the workspace may share no byte
+ * with one another or with what is read (judged as for emb_paged_store). A cache of 16-bit type has q's type. */
 typedef struct {
     const void* q; /* [requests, heads, dim], q_stride = request, head */
     void* out;

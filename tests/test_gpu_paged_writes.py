@@ -1,4 +1,4 @@
-"""What the paged-cache operators write into, as autograd sees it."""
+"""What the paged-cache operators write into, as autograd sees it, and in which memory."""
 
 import pytest
 import torch
@@ -78,3 +78,49 @@ def test_tensors_of_inference_mode_are_taken_in_and_out_of_it(paged):
     with torch.inference_mode():
         paged.attend(**plain)
     assert plain["out"]._version > 0 and arguments["out"].is_inference()
+
+
+@pytest.mark.parametrize("lengths, heads, kv_heads, dim, cache", [
+    ([5000, 17, 0, 900, 12000], 8, 2, 128, F16), ([9000, 0, 7, 5000, 8000] * 12, 32, 8, 128, F16), ([40, 3, 100], 4, 2, 64, F16), ([9000, 0, 17, 12000] * 20, 16, 4, 64, torch.float8_e4m3fn),
+    ([700] * 50, 40, 1, 256, F16)])
+def test_attend_puts_its_result_where_the_queries_were(paged, lengths, heads, kv_heads, dim, cache):
+    """Heads that are cut, whole, shared by warps and side by side, and groups of more rows than a block has."""
+    s = make_attend(lengths, heads, kv_heads, dim, F16, cache, 16)
+    want = paged.attend(**s)
+    wide = torch.full((len(lengths), heads + 3, dim), 5.0, dtype=F16, device="cuda")
+    for queries in (s["q"].clone(), wide[:, 1:heads + 1].copy_(s["q"])):
+        got = paged.attend(**(s | dict(q=queries, out=queries)))
+        assert got.data_ptr() == queries.data_ptr() and torch.equal(queries, want)
+    assert bool((wide[:, 0] == 5).all()) and bool((wide[:, heads + 1:] == 5).all())
+
+
+def test_attend_refuses_a_workspace_that_something_else_is(paged):
+    """Through the C entry: the workspace over out, lse, the queries or the pages, wholly or by its last bytes."""
+    from emmy_ptx import driver
+    from test_paged import ATTEND
+    import ctypes
+    library = driver.library()
+    library.emb_paged_attend.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+    library.emb_paged_attend_workspace.argtypes, library.emb_paged_attend_workspace.restype = [ctypes.c_char_p], ctypes.c_int64
+    s = attend_arguments()
+    s["table"] = s["table"].contiguous()
+    arena = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+
+    def fields(workspace, size, width=1000):
+        k, v = s["k_pages"], s["v_pages"]
+        return ATTEND.pack(s["q"].data_ptr(), s["out"].data_ptr(), s["lse"].data_ptr(), s["table"].data_ptr(), s["lengths"].data_ptr(), workspace,
+                           k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], k.shape[0], 16, 2, 64, 1, 1.0, 1.0, 0, 256, 64, 256, 64, s["table"].shape[1], size, 2, 4,
+                           width, 1, 0, 0.125)
+
+    need = library.emb_paged_attend_workspace(fields(0, 0))  # (a table row this wide is never reached by these lengths)
+    assert 0 < need < arena.numel()
+    s["table"] = torch.zeros(2, 1000, dtype=torch.int32, device="cuda")
+    s["out"] = arena[need:].view(F16)[:2 * 4 * 64].view(2, 4, 64)
+    s["lse"] = arena[-4096:].view(torch.float32)[:8].view(2, 4)
+    for workspace, which in ((arena.data_ptr() + 16, "out and the workspace"), (s["lse"].data_ptr() - need + 16, "lse and the workspace"),
+                             (s["q"].data_ptr(), "the workspace and "), (s["k_pages"].data_ptr() - need + 16, "the workspace and ")):
+        assert library.emb_paged_attend(fields(workspace, need), None) == -2
+        text = library.emb_last_error().decode()
+        assert text.startswith("paged_attend: " + which) and text.endswith("share memory"), text
+    assert library.emb_paged_attend(fields(arena.data_ptr(), need), torch.cuda.current_stream().cuda_stream) == 0  # it ends where out begins
+    torch.cuda.synchronize()

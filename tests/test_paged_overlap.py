@@ -122,3 +122,34 @@ def test_store_takes_memory_that_is_apart(changes):
 @pytest.mark.parametrize("changes, match", STORE_TOUCH)
 def test_store_refuses_memory_that_it_writes_and_reads(changes, match):
     assert Call("store", STORE).text(store_fields(**changes)) == f"paged_store: {match} share memory"
+
+
+# ---- attend: 3 requests of 4 heads of 64 over 2 key heads, a table of 2 pages a request
+
+LSE, TABLE, WS = (x << 20 for x in range(8, 11))
+
+
+def attend_fields(cache=(), **changes):
+    cache = dict(dict(k=KP, v=VP), **dict(cache))
+    return flat(dict(q=Q, out=OUT, lse=LSE, table=TABLE, lengths=TABLE + 4096, ws=WS, cache=cache_fields(**cache), q0=256, q1=64, o0=256, o1=64, ts=2, wb=1 << 19, requests=3,
+                     heads=4, width=2, dtype=1, window=0, scale=0.125), changes)
+
+
+ATTEND_APART = [
+    dict(), dict(out=Q), dict(q0=512, o0=512, out=Q + 512), dict(lse=0), dict(cache=dict(v=KP)), dict(cache=PAIRS), dict(ts=0), dict(out=TABLE + 8192, lse=TABLE + 64),
+    dict(out=Q + 3 * 512, lse=Q + 6 * 512), dict(requests=1, q0=0, o0=0, ts=2, out=Q), dict(ts=16, lse=TABLE + 2048), dict(q0=0, out=Q + 512), dict(cache=dict(ks0=4096, ks1=256), out=KP + 2 ** 19)]
+ATTEND_TOUCH = [
+    (dict(out=Q + 128), "out and q"), (dict(out=Q + 512), "out and q"), (dict(q0=512, o0=512, out=Q + 384), "out and q"), (dict(q0=0, out=Q), "out and q"), (dict(q1=128, q0=512, out=Q), "out and q"),
+    (dict(out=KP), "out and the keys' pages"), (dict(out=VP + 16368), "out and the values' pages"), (dict(out=TABLE - 1520), "out and table"), (dict(out=TABLE + 4096), "out and lengths"),
+    (dict(lse=OUT + 1532), "out and lse"), (dict(lse=Q), "lse and q"), (dict(lse=KP + 4), "lse and the keys' pages"), (dict(lse=TABLE + 20), "lse and table"), (dict(lse=TABLE + 4096 - 44), "lse and lengths"),
+    (dict(ts=4, lse=TABLE + 4), "lse and table")]
+
+
+@pytest.mark.parametrize("changes", ATTEND_APART)
+def test_attend_takes_memory_that_is_apart(changes):
+    assert "cannot be asked for its SMs" in Call("attend", ATTEND).text(attend_fields(**changes))
+
+
+@pytest.mark.parametrize("changes, match", ATTEND_TOUCH)
+def test_attend_refuses_memory_that_it_writes_and_reads(changes, match):
+    assert Call("attend", ATTEND).text(attend_fields(**changes)) == f"paged_attend: {match} share memory"
