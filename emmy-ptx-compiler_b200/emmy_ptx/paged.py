@@ -52,7 +52,8 @@ def assign(cached, fresh, table, free_pages, free_head, page_size: int, tokens: 
     place. ``free_pages`` [n] are handed out from entry ``free_head`` [1] on. ``tokens``: the step's rows, at least as
     many as there are new tokens. All int32. Returns slots and positions [tokens] (-1 and 0 behind the last request),
     starts [requests + 1], lengths [requests], free_head [1] and report [4] (pages taken, requests refused, rows wanted
-    beyond ``tokens``, rows wanted); ``out``: these six tensors, to be written instead of new ones. A request whose tokens
+    beyond ``tokens``, rows wanted); ``out``: these six tensors, to be written instead of new ones (in memory that
+    is none of the inputs' and not shared). A request whose tokens
     fit neither its table row nor the step nor the free pages is refused whole: slots -1, length and table as they were.
     """
     if out is not None and type(out) is not Assigned:

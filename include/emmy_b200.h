@@ -231,7 +231,8 @@ typedef struct {
  * step's `tokens` rows, or when the free pages end before its need and the need of
  * the requests before it: its slots are -1, its length stays cached[b], its table
  * row stays as it is. An entry of the table that is negative gives slot -1.
- * Outputs may not share memory with inputs (but for `table`). */
+ * Outputs and `table` may share no byte with one another or with the inputs (judged
+ * as for emb_paged_store). */
 typedef struct {
     const int32_t* cached;
     const int32_t* fresh;

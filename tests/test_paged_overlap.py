@@ -1,7 +1,7 @@
 """Memory that an operator of the paged cache would write while it reads it, or write twice: refused by the host.
 
 The calls here carry addresses that no launch may ever see, so they run only where no GPU can: an accepted call ends at the
-question for the device's SMs.
+question for the device's SMs, or at the launch.
 """
 
 import ctypes
@@ -153,3 +153,39 @@ def test_attend_takes_memory_that_is_apart(changes):
 @pytest.mark.parametrize("changes, match", ATTEND_TOUCH)
 def test_attend_refuses_memory_that_it_writes_and_reads(changes, match):
     assert Call("attend", ATTEND).text(attend_fields(**changes)) == f"paged_attend: {match} share memory"
+
+
+# ---- assign: 3 requests, a table of 4 pages a request, 9 free pages, 8 rows
+
+
+def assign_fields(**changes):
+    at = {name: (1 << 20) + 4096 * i for i, name in enumerate(("cached", "fresh", "table", "free", "head", "slots", "positions", "starts", "lengths", "head_out", "report"))}
+    return flat(dict(at, ts=4, requests=3, width=4, count=9, size=16, tokens=8, r=0), changes)
+
+
+def place(name, offset=0):
+    names = ("cached", "fresh", "table", "free", "head", "slots", "positions", "starts", "lengths", "head_out", "report")
+    return (1 << 20) + 4096 * names.index(name) + offset
+
+
+ASSIGN_APART = [
+    dict(), dict(fresh=place("cached")), dict(head=place("cached", 8)), dict(free=place("fresh")), dict(positions=place("slots", 32)), dict(starts=place("slots", 32), lengths=place("slots", 48)),
+    dict(head_out=place("report", 16)), dict(ts=16, slots=place("table", 16), positions=place("table", 80)) | dict(tokens=8), dict(requests=0, cached=0, fresh=0, table=0, lengths=0),
+    dict(tokens=0, slots=place("report"), positions=place("report")), dict(count=0, free=place("slots"))]
+ASSIGN_TOUCH = [
+    (dict(slots=place("positions")), "slots and positions"), (dict(slots=place("positions", 28)), "slots and positions"), (dict(starts=place("lengths", -12)), "starts and lengths"),
+    (dict(lengths=place("cached", 4)), "lengths and cached"), (dict(lengths=place("fresh", -8)), "lengths and fresh"), (dict(table=place("free")), "table and free_pages"),
+    (dict(table=place("slots", 16)), "table and slots"), (dict(ts=16, slots=place("table", 36)), "table and slots"), (dict(head_out=place("report", 12)), "free_head_out and report"),
+    (dict(head_out=place("free", 8)), "free_head_out and free_pages"), (dict(report=place("head", -12)), "report and free_head"), (dict(starts=place("head", -12)), "starts and free_head"),
+    (dict(positions=place("fresh", 8)), "positions and fresh"), (dict(slots=place("free", 32)), "slots and free_pages"), (dict(table=place("head")), "table and free_head")]
+
+
+@pytest.mark.parametrize("changes", ASSIGN_APART)
+def test_assign_takes_memory_that_is_apart(changes):
+    text = Call("assign", ASSIGN).text(assign_fields(**changes))
+    assert text.startswith("launch of paged_assign: "), text  # without a device
+
+
+@pytest.mark.parametrize("changes, match", ASSIGN_TOUCH)
+def test_assign_refuses_memory_that_it_writes_and_reads(changes, match):
+    assert Call("assign", ASSIGN).text(assign_fields(**changes)) == f"paged_assign: {match} share memory"
