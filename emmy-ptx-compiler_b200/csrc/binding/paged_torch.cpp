@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -169,7 +170,8 @@ int device_of(const char* who, std::initializer_list<Arg> all) {
 // a tensor that wants its gradient would silently get none (and one that is written would lose what it had); so would the
 // tangent of forward differentiation, which torch.no_grad() does not end
 void no_graph(const char* who, std::initializer_list<Arg> all) {
-    const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    const bool backward = c10::GradMode::is_enabled();
+    const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0);  // (a level is open)
     for (const Arg& x : all) {
         if (!x.given()) continue;
         if (backward && x->requires_grad()) refuse("%s: %s requires a gradient, and this operator has none (call it under torch.no_grad())", who, x.name);

@@ -173,9 +173,9 @@ extern "C" int emb_paged_assign(const emb_paged_assign_t* args, void* stream) {
     if (a.requests > 1 && a.table_stride < a.table_width) return refuse("paged_assign: rows of the table overlap");
     if (a.lengths && (a.lengths == a.cached || a.lengths == a.fresh)) return refuse("paged_assign: lengths may not be cached or fresh");
     if (a.free_head_out == a.free_head) return refuse("paged_assign: free_head_out may not be free_head");
-    const auto ints = [](const char* name, const void* p, int64_t n) { return Area(name, p, wide(n) * 4); };
+    const auto ints = [](const char* name, const void* p, int64_t n) { return Area(name, p, n * 4); };
     const int64_t requests = a.requests;
-    const Area written[7] = {ints("table", a.table, requests ? a.table_width : 0).by(requests, wide(a.table_stride) * 4), ints("slots", a.slots, a.tokens), ints("positions", a.positions, a.tokens),
+    const Area written[7] = {ints("table", a.table, requests ? a.table_width : 0).by(requests, a.table_stride * 4), ints("slots", a.slots, a.tokens), ints("positions", a.positions, a.tokens),
                              ints("starts", a.starts, requests + 1), ints("lengths", a.lengths, requests), ints("free_head_out", a.free_head_out, 1), ints("report", a.report, 4)};
     const Area read[4] = {ints("cached", a.cached, requests), ints("fresh", a.fresh, requests), ints("free_pages", a.free_pages, a.free_count), ints("free_head", a.free_head, 1)};
     const char* which[2];

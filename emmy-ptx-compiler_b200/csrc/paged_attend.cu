@@ -41,6 +41,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <optional>
 
 #include "emb_frag.cuh"
 
@@ -871,19 +872,27 @@ template <class Cfg> int grid_of(const emb_paged_attend_t& a, int sms) {
     return most < all ? static_cast<int>(most) : all;
 }
 
-// (out may be q: a head's queries are in registers before its output is written, by the CTA that has the head to itself or by
-// the join.) `workspace`: its bytes, where the call has been found to need one
-int check_overlap(const emb_paged_attend_t& a, int64_t workspace) {
-    const Area written[3] = {rows_at("out", a.out, a.requests, a.heads, a.cache.dim, a.out_stride), Area("lse", a.lse, wide(a.requests) * a.heads * 4),
-                             Area("the workspace", workspace ? a.workspace : nullptr, workspace)};
-    const Area read[5] = {rows_at("q", a.q, a.requests, a.heads, a.cache.dim, a.q_stride), pages_at("the keys' pages", a.cache, a.cache.k, a.cache.k_stride),
-                          pages_at("the values' pages", a.cache, a.cache.v, a.cache.v_stride),
-                          Area("table", a.table, wide(a.table_width) * 4).by(a.requests, wide(a.table_stride) * 4), Area("lengths", a.lengths, wide(a.requests) * 4)};
-    const char* which[2];
-    return touches(written, read, &read[0], which) ? refuse("paged_attend: %s and %s share memory", which[0], which[1]) : 0;
-}
+// What a call writes and reads, but for the workspace, whose bytes are known later. (out may be q: a head's queries are in
+// registers before its output is written, by the CTA that has the head to itself or by the join.)
+struct Memory {
+    Area written[2], read[5];
+    explicit Memory(const emb_paged_attend_t& a)
+        : written{rows_at("out", a.out, a.requests, a.heads, a.cache.dim, a.out_stride), Area("lse", a.lse, int64_t(a.requests) * a.heads * 4)},
+          read{rows_at("q", a.q, a.requests, a.heads, a.cache.dim, a.q_stride), pages_at("the keys' pages", a.cache, a.cache.k, a.cache.k_stride),
+               pages_at("the values' pages", a.cache, a.cache.v, a.cache.v_stride), Area("table", a.table, int64_t(a.table_width) * 4).by(a.requests, a.table_stride * 4),
+               Area("lengths", a.lengths, int64_t(a.requests) * 4)} {}
+    int refuse_shared() const {
+        const char* which[2];
+        return touches(written, read, &read[0], which) ? refuse("paged_attend: %s and %s share memory", which[0], which[1]) : 0;
+    }
+    int refuse_shared(const void* workspace, int64_t bytes) const {
+        const Area w[1] = {Area("the workspace", workspace, bytes)};
+        const char* which[2];
+        return touches(w, written, nullptr, which) || touches(w, read, nullptr, which) ? refuse("paged_attend: %s and %s share memory", which[0], which[1]) : 0;
+    }
+};
 
-template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {
+template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a, const Memory* memory, cudaStream_t stream, int64_t* need) {
     using Cfg = Config<T, C, DIM, HT>;
     const int sms = sm_count();
     if (!sms) return refuse("paged_attend: the current device cannot be asked for its SMs");
@@ -903,7 +912,7 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
     }
     if (bytes && (a.workspace_bytes < bytes || !a.workspace || !aligned16(a.workspace)))
         return refuse("paged_attend: a workspace of %lld bytes (16-byte aligned) is needed, not %lld", static_cast<long long>(bytes), static_cast<long long>(a.workspace_bytes));
-    if (int r = bytes ? check_overlap(a, bytes) : 0) return r;
+    if (int r = bytes ? memory->refuse_shared(a.workspace, bytes) : 0) return r;
     auto kernel = paged_attend_kernel<T, C, DIM, HT>;
     static std::atomic<bool> sized[MAX_DEVICES];  // (threads that race here set the same value)
     int device = 0;
@@ -926,14 +935,14 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
                                                    Divisor(rows), static_cast<uint32_t>(units), split));
 }
 
-template <class T, class C> int run_dim(const emb_paged_attend_t& a, cudaStream_t stream, int64_t* need) {
+template <class T, class C> int run_dim(const emb_paged_attend_t& a, const Memory* memory, cudaStream_t stream, int64_t* need) {
     // a group of more query heads than a CTA's rows is cut into several, which read the same keys (at about the same time, so
     // from L2): 32 query heads of 128 in one CTA need more registers than it has, and took 75 us where two of 16 take 50
     const int group = a.heads / a.cache.kv_heads;
     switch (a.cache.dim) {
-        case 64: return group <= 8 ? run<T, C, 64, 1>(a, stream, need) : run<T, C, 64, 2>(a, stream, need);
-        case 128: return group <= 8 ? run<T, C, 128, 1>(a, stream, need) : run<T, C, 128, 2>(a, stream, need);
-        default: return run<T, C, 256, 1>(a, stream, need);
+        case 64: return group <= 8 ? run<T, C, 64, 1>(a, memory, stream, need) : run<T, C, 64, 2>(a, memory, stream, need);
+        case 128: return group <= 8 ? run<T, C, 128, 1>(a, memory, stream, need) : run<T, C, 128, 2>(a, memory, stream, need);
+        default: return run<T, C, 256, 1>(a, memory, stream, need);
     }
 }
 
@@ -950,6 +959,7 @@ int attend(const emb_paged_attend_t* args, void* stream, int64_t* need) {
     if (!(a.scale > -INFINITY && a.scale < INFINITY)) return refuse("paged_attend: the scale is not a finite number");
     if (need) *need = 0;
     if (a.requests == 0) return 0;
+    std::optional<Memory> memory;  // (of a call for the size alone it is not looked at)
     if (!need) {
         if (!a.table || !a.lengths) return refuse("paged_attend: null table or lengths");
         if (!a.q || !a.out || !aligned16(a.q) || !aligned16(a.out)) return refuse("paged_attend: q or out is null or not 16-byte aligned");
@@ -957,11 +967,11 @@ int attend(const emb_paged_attend_t* args, void* stream, int64_t* need) {
             if (!stride_fits(s[0], 2) || !stride_fits(s[1], 2)) return refuse("paged_attend: a stride of q or out is not a multiple of 16 bytes below 2^32 elements");
         const int64_t rows[2] = {a.requests, a.heads};
         if (!rows_apart(rows, a.out_stride, a.cache.dim)) return refuse("paged_attend: rows of out overlap");
-        if (int r = check_overlap(a, 0)) return r;
+        if (int r = memory.emplace(a).refuse_shared()) return r;
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a.dtype == EMB_F16) return a.cache.dtype == EMB_U8 ? run_dim<__half, E4m3>(a, s, need) : run_dim<__half, __half>(a, s, need);
-    return a.cache.dtype == EMB_U8 ? run_dim<__nv_bfloat16, E4m3>(a, s, need) : run_dim<__nv_bfloat16, __nv_bfloat16>(a, s, need);
+    if (a.dtype == EMB_F16) return a.cache.dtype == EMB_U8 ? run_dim<__half, E4m3>(a, memory ? &*memory : nullptr, s, need) : run_dim<__half, __half>(a, memory ? &*memory : nullptr, s, need);
+    return a.cache.dtype == EMB_U8 ? run_dim<__nv_bfloat16, E4m3>(a, memory ? &*memory : nullptr, s, need) : run_dim<__nv_bfloat16, __nv_bfloat16>(a, memory ? &*memory : nullptr, s, need);
 }
 
 }  // namespace

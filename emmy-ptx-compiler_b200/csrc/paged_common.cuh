@@ -76,11 +76,11 @@ inline int check_cache(const char* who, const emb_paged_cache_t& c, int q_dtype)
 
 // rows [n, heads, dim] of 16 bits, and the pages of a cache
 inline Area rows_at(const char* name, const void* p, int64_t n, int heads, int dim, const int64_t (&stride)[2]) {
-    return Area(name, p, dim * 2).by(heads, wide(stride[1]) * 2).by(n, wide(stride[0]) * 2);
+    return Area(name, p, dim * 2).by(heads, stride[1] * 2).by(n, stride[0] * 2);
 }
 inline Area pages_at(const char* name, const emb_paged_cache_t& c, const void* p, const int64_t (&stride)[3]) {
     const int size = c.dtype == EMB_U8 ? 1 : 2;
-    return Area(name, p, c.dim * size).by(c.kv_heads, wide(stride[2]) * size).by(c.page_size, wide(stride[1]) * size).by(c.pages, wide(stride[0]) * size);
+    return Area(name, p, c.dim * size).by(c.kv_heads, stride[2] * size).by(c.page_size, stride[1] * size).by(c.pages, stride[0] * size);
 }
 
 constexpr int MAX_DEVICES = 64;

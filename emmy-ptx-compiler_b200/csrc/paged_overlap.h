@@ -13,16 +13,18 @@ namespace paged {
 using wide = __int128;  // a 31-bit count times a 34-bit stride
 
 struct Area {
-    const char* name = "";
-    wide at = 0, run = 0, last = 0;  // first byte, bytes of a run, the last run's first byte from `at`
+    const char* name;
+    uint64_t at;
+    int64_t run;  // bytes of one
+    wide end;     // behind the last byte
     int n = 0;
-    wide count[3] = {}, stride[3] = {};  // runs, and bytes from one to the next
+    int64_t count[3], stride[3];  // runs, and bytes from one to the next (the first n)
 
-    Area(const char* name_, const void* p, wide run_) : name(name_), at(reinterpret_cast<uintptr_t>(p)), run(p ? run_ : 0) {}
+    Area(const char* name_, const void* p, int64_t run_) : name(name_), at(reinterpret_cast<uintptr_t>(p)), run(p ? run_ : 0), end(wide(at) + run) {}
     // (a stride of 0 repeats a run; no runs at all are no area)
-    Area& by(wide c, wide s) {
+    Area& by(int64_t c, int64_t s) {
         if (c < 1) run = 0;
-        if (c > 1 && s > 0) count[n] = c, stride[n] = s, ++n, last += (c - 1) * s;
+        if (c > 1 && s > 0) count[n] = c, stride[n] = s, ++n, end += wide(c - 1) * s;
         return *this;
     }
     bool same(const Area& b) const {
@@ -51,8 +53,7 @@ inline bool reaches(const Steps* s, int n, wide lo, wide hi, int& looks) {
     return false;
 }
 
-inline bool touch(const Area& a, const Area& b) {
-    if (a.run <= 0 || b.run <= 0 || a.at + a.last + a.run <= b.at || b.at + b.last + b.run <= a.at) return false;
+inline bool runs_touch(const Area& a, const Area& b) {
     Steps s[6];
     int n = 0;
     const auto add = [&](wide stride, wide back, wide ahead) {
@@ -67,10 +68,14 @@ inline bool touch(const Area& a, const Area& b) {
     };
     for (int i = 0; i < a.n; ++i) add(a.stride[i], 0, a.count[i] - 1);
     for (int i = 0; i < b.n; ++i) add(b.stride[i], b.count[i] - 1, 0);
-    // run i of a is at a.at + x, run j of b at b.at + y, and x - y is such a sum: they meet where b.at - a.at - a.run < x - y < b.at - a.at + b.run
+    // run i of a is at a.at + x, run j of b at b.at + y, and x - y is such a sum: they meet where
+    // b.at - a.at - a.run < x - y < b.at - a.at + b.run
     int looks = 4096;
-    return reaches(s, n, b.at - a.at - a.run, b.at - a.at + b.run, looks);
+    const wide ahead = wide(b.at) - wide(a.at);
+    return reaches(s, n, ahead - a.run, ahead + b.run, looks);
 }
+
+inline bool touch(const Area& a, const Area& b) { return a.end > b.at && b.end > a.at && a.run > 0 && b.run > 0 && runs_touch(a, b); }
 
 // the first of `written` that touches another of them or one of `read` (which: the names), but for a pair that is `allowed` where
 // it is the same area

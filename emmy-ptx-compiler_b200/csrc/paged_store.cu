@@ -192,12 +192,13 @@ extern "C" int emb_paged_store(const emb_paged_store_t* args, void* stream) {
     const int64_t rows[2] = {a.tokens, a.heads}, slots[3] = {a.cache.pages, a.cache.page_size, a.cache.kv_heads};
     if (!rows_apart(rows, a.out_stride, a.cache.dim)) return refuse("paged_store: rows of q_out overlap");
     if (!rows_apart(slots, a.cache.k_stride, a.cache.dim) || !rows_apart(slots, a.cache.v_stride, a.cache.dim)) return refuse("paged_store: slots of the cache overlap");
-    const int n = a.tokens, kv_heads = a.cache.kv_heads, dim = a.cache.dim;
+    const int64_t n = a.tokens;
+    const int kv_heads = a.cache.kv_heads, dim = a.cache.dim;
     const Area written[3] = {rows_at("q_out", a.q_out, n, a.heads, dim, a.out_stride), pages_at("the keys' pages", a.cache, a.cache.k, a.cache.k_stride),
                              pages_at("the values' pages", a.cache, a.cache.v, a.cache.v_stride)};
     const Area read[8] = {rows_at("q", a.q, n, a.heads, dim, a.q_stride), rows_at("k", a.k, n, kv_heads, dim, a.k_stride), rows_at("v", a.v, n, kv_heads, dim, a.v_stride),
-                          Area("slots", a.slots, n * wide(4)), Area("positions", a.rot ? a.positions : nullptr, n * wide(4)),
-                          Area("rope", a.rot ? a.rope : nullptr, wide(a.rope_rows) * a.rot * 4), Area("q_weight", a.q_weight, dim * 2), Area("k_weight", a.k_weight, dim * 2)};
+                          Area("slots", a.slots, n * 4), Area("positions", a.rot ? a.positions : nullptr, n * 4),
+                          Area("rope", a.rot ? a.rope : nullptr, int64_t(a.rope_rows) * a.rot * 4), Area("q_weight", a.q_weight, dim * 2), Area("k_weight", a.k_weight, dim * 2)};
     const char* which[2];
     if (touches(written, read, &read[0], which)) return refuse("paged_store: %s and %s share memory", which[0], which[1]);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -117,7 +117,7 @@ def test_attend_refuses_a_workspace_that_something_else_is(paged):
     s["table"] = torch.zeros(2, 1000, dtype=torch.int32, device="cuda")
     s["out"] = arena[need:].view(F16)[:2 * 4 * 64].view(2, 4, 64)
     s["lse"] = arena[-4096:].view(torch.float32)[:8].view(2, 4)
-    for workspace, which in ((arena.data_ptr() + 16, "out and the workspace"), (s["lse"].data_ptr() - need + 16, "lse and the workspace"),
+    for workspace, which in ((arena.data_ptr() + 16, "the workspace and out"), (s["lse"].data_ptr() - need + 16, "the workspace and lse"),
                              (s["q"].data_ptr(), "the workspace and "), (s["k_pages"].data_ptr() - need + 16, "the workspace and ")):
         assert library.emb_paged_attend(fields(workspace, need), None) == -2
         text = library.emb_last_error().decode()
