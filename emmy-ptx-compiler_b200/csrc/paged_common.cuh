@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <cfloat>
 #include <cstdarg>
 #include <cstdio>
 
@@ -70,7 +71,11 @@ inline int check_cache(const char* who, const emb_paged_cache_t& c, int q_dtype)
     for (int i = 0; i < 3; ++i)
         if (!stride_fits(c.k_stride[i], size) || !stride_fits(c.v_stride[i], size))
             return refuse("%s: a stride of the pages is not a multiple of 16 bytes below 2^32 elements", who);
-    if (!(c.k_scale > 0.f) || !(c.v_scale > 0.f) || c.k_scale > 3.0e38f || c.v_scale > 3.0e38f) return refuse("%s: a cache scale is not a positive number", who);
+    for (const float scale : {c.k_scale, c.v_scale}) {
+        // (of a subnormal number the reciprocal may be infinite)
+        if (!(scale >= FLT_MIN && scale <= 3.0e38f)) return refuse("%s: a cache scale of %g is not a positive number between 1.2e-38 and 3e38", who, static_cast<double>(scale));
+        if (c.dtype != EMB_U8 && scale != 1.f) return refuse("%s: scales belong to a cache of e4m3 codes", who);
+    }
     return 0;
 }
 
