@@ -54,7 +54,7 @@ inline bool reaches(const Steps* s, int n, wide lo, wide hi, int& looks) {
 }
 
 inline bool runs_touch(const Area& a, const Area& b) {
-    Steps s[6];
+    Steps s[6] = {};
     int n = 0;
     const auto add = [&](wide stride, wide back, wide ahead) {
         int i = 0;

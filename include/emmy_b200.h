@@ -209,7 +209,7 @@ typedef struct {
     int32_t kv_heads;
     int32_t dim;     /* 64, 128 or 256 */
     int32_t dtype;   /* EMB_F16, EMB_BF16, or EMB_U8: e4m3 codes */
-    float k_scale;   /* of e4m3 codes: value = code * scale; else 1 */
+    float k_scale;   /* of e4m3 codes: value = code * scale, 1.2e-38 to 3e38; else 1 */
     float v_scale;
     int32_t reserved; /* 0 */
 } emb_paged_cache_t;
@@ -227,6 +227,8 @@ typedef struct {
  *   free_head_out            *free_head + pages taken
  *   report[4]                pages taken, requests refused, rows wanted beyond
  *                            `tokens`, rows wanted
+ * Sums of counts stop at 2^31 - 1: starts, positions and the rows wanted are never
+ * more, and rows wanted beyond `tokens` are those up to there.
  * A request is refused whole when its tokens do not fit its table row or the
  * step's `tokens` rows, or when the free pages end before its need and the need of
  * the requests before it: its slots are -1, its length stays cached[b], its table
