@@ -9,7 +9,7 @@
 // Products are mma.sync m16n8k16 with the KEYS as rows: S^T = K Q^T (16 keys x 8 query heads) and O^T = V^T P^T (16 dims x
 // 8 heads), so a group of up to eight heads wastes no row, and S^T becomes the operand P^T by one 8 x 8 transposition
 // (movmatrix). tcgen05 would want 128 rows of one request and head at a time in shared memory as it lays them out; the
-// tensor work here is a tenth of what the legacy path does in the time HBM needs for the bytes. A WARP owns KEYS
+// tensor work here is a seventh of what the legacy path does in the time HBM needs for the bytes. A WARP owns KEYS
 // consecutive keys at a time: it copies them into a ring of its own with cp.async (rows found through the page table, so any
 // page size and any strides; rows behind the length are filled with zeros and not read), multiplies, and keeps a maximum,
 // sum and output of its own. No barrier stands between copies and products.
@@ -23,7 +23,8 @@
 // A weight is two 16-bit numbers and so two products with the values (`split`). One alone is off by as much as the result's own
 // rounding: the mean error against 64 bits was 1.3 times that of a result rounded once. The second product costs under 1 %
 // where HBM is the bound (8 x 4096 keys 87.6 -> 88.1, 64 ragged requests 168.1 -> 168.8 us), 4 % over e4m3 codes with f16 queries
-// and 8 % with 16 query heads of 128 a key head (64 requests up to 4000 keys: 57.4 -> 62.1 us).
+// and 8 to 13 % with 16 query heads and more of 128 a key head (64 requests up to 4000 keys: 57.5 -> 62.3 us with 64 on 4 key
+// heads, 48.1 -> 54.3 with 64 on 2), whatever the order of the products.
 //
 // The work is cut by TILES, all requests and heads (or sets of heads side by side) behind one another: CTA c of n takes
 // tiles [c T / n, (c + 1) T / n), whatever their requests. So a single long request and a ragged batch both spread evenly, and
@@ -33,9 +34,12 @@
 // Measured (a pass among others, join included; of the measured copy rate of 6.55 TB/s): 8 requests x 4096 keys x 32 key heads
 // of 128, f16, 537 MB: 88 us, 0.93 (the kernel alone 83 us, 0.99); 64 ragged requests up to 8192 keys, 32 query heads on 8 key
 // heads, bf16, 1070 MB: 169 us, 0.97; one request of 131072 keys, 537 MB: 90 us, 0.91; 128 requests of up to 2000 keys, 64
-// query heads on 8 key heads of 64, e4m3, 224 MB: 55 us, 0.62 (the decode of the codes: 45 % of the issue slots, with three
-// warps a scheduler to fill them; rows of 64 bytes come at 5 to 6.3 TB/s whatever reads them). Small calls are bound by latency:
-// 5.9 us for one request of 113 keys, 8 where pieces are joined.
+// query heads on 8 key heads of 64, e4m3, 224 MB: 55 us, 0.62 (the codes' decode and a row's bookkeeping: 46 % of the issue slots,
+// with three warps a scheduler to fill them; rows of 64 bytes come at 5 to 6.3 TB/s whatever reads them). Small calls are bound
+// by latency: 6.2 us for one request of 113 keys, 8 where pieces are joined.
+// Farther from one reading of the bytes (us, and us at the copy rate): groups of more than eight query heads (62 / 38: 64 requests
+// up to 4000 keys, 64 on 4 heads of 128), e4m3 of 128 and 256 (52 / 38, 38 / 19), calls of 10 to 150 MB (30 / 18: 56 requests up
+// to 8000 keys, one key head of 128; about 8 us are fixed), many requests of few keys at 256 dims (13: 115 of 2 keys, 5 heads).
 
 #include "paged_common.cuh"
 
@@ -936,8 +940,10 @@ template <class T, class C, int DIM, int HT> int run(const emb_paged_attend_t& a
 }
 
 template <class T, class C> int run_dim(const emb_paged_attend_t& a, const Memory* memory, cudaStream_t stream, int64_t* need) {
-    // a group of more query heads than a CTA's rows is cut into several, which read the same keys (at about the same time, so
-    // from L2): 32 query heads of 128 in one CTA need more registers than it has, and took 75 us where two of 16 take 50
+    // a group of more query heads than a CTA's rows is cut into several, which read the same keys: 32 query heads of 128 in one
+    // CTA need more registers than it has, and took 75 us where two of 16 took 50. Those are heads of their own in the order of
+    // the tiles, a whole head apart, so unless they stand side by side HBM delivers the keys once for each: 64 requests up to
+    // 4000 keys, 64 on 2 heads, take 54 us where one reading takes 19
     const int group = a.heads / a.cache.kv_heads;
     switch (a.cache.dim) {
         case 64: return group <= 8 ? run<T, C, 64, 1>(a, memory, stream, need) : run<T, C, 64, 2>(a, memory, stream, need);

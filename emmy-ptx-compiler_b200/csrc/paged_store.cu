@@ -12,8 +12,11 @@
 // next AHEAD of them loaded while AHEAD are at work, and has the brackets, the slot and the addresses ready for all of them. A group has heads of one
 // kind only (q, k or v). Measured on 16384 tokens of 32 + 8 + 8 heads of 128, bf16, 407 MB: 79 us = 5.15 TB/s, 0.79 of the
 // measured copy rate (with the elements in order, the partners fetched by shuffles and heads of all kinds in a group: 130 us;
-// 16-byte pieces of half as many lanes: 101; packed f32x2 arithmetic: no change, so it is not the arithmetic that bounds it
-// now but reads and 256-byte row writes mixed in HBM). Small steps are bound by the launch: 4.1 us a call for 8 to 256 tokens.
+// 16-byte pieces of half as many lanes: 101; packed f32x2 arithmetic: no change). Two thirds of the issue slots are taken, by
+// addresses, conversions and shuffles as much as by arithmetic, and reads and 256-byte row writes are mixed in HBM; which of the
+// two is the bound has not been told apart. Into an e4m3 cache: 72 us, 0.79. With few heads a group's start is a larger part (slot
+// or position, then angles and weight, before the first store, and nothing of the next group's meanwhile): 10456 tokens of 8 + 8 +
+// 8 heads of 128, f16, 133 MB: 36 us, 0.57. Small steps are bound by the launch: 4.5 us a call for 8 to 1001 tokens.
 
 #include <algorithm>
 

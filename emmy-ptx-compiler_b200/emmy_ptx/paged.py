@@ -3,7 +3,9 @@
 Library operators of libemmyb200.so (include/emmy_b200.h states each in full) on torch tensors, with run-time sizes: one
 step of a server calls ``assign`` once (pages and slots for the step's new tokens, from the requests' lengths), and in
 each layer ``store`` (norm and rotation of the new queries and keys; keys and values into their slots) and ``attend``
-(one new token of each request over its pages). Prompts' own rows go through the attention family.
+(one new token of each request over its pages). There is no attention of several new tokens of a request over its pages: a
+prompt's own goes through the attention family, from keys that the caller norms and rotates as ``store`` does (it returns the
+queries only), and a prompt piece on top of cached tokens has none.
 
 Calls run on the current stream of the tensors' device, which need not be the current one, read nothing back and may be
 captured into a CUDA graph. Arguments that the host can judge are refused with ``driver.EmbError`` (code -2). There is no

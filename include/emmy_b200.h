@@ -185,7 +185,9 @@ typedef struct {
  * emb_paged_assign gives the step's new tokens their places in the cache,
  * emb_paged_store normalises and rotates the new queries and keys and stores keys
  * and values there, emb_paged_attend attends one new token of each request over
- * its pages (a prompt's own rows go through the attention family).
+ * its pages. Attention of several new tokens of a request over its pages there is
+ * none: a prompt's own goes through the attention family, from dense keys that the
+ * caller has normalised and rotated (emb_paged_store returns the queries only).
  *
  * Every pointer is a device address on the current device; the caller owns all of
  * them. Strides are in elements. Calls are asynchronous on `stream`, allocate
